@@ -22,6 +22,8 @@
 #include "grouped_gemm_2sm.cuh"
 #include "quantize.cuh"
 #include "moe.cuh"
+#include "gemv.cuh"
+#include "norm.cuh"
 
 // Fixed split-K scratch of the allocation-free dual GEMM entry point
 // (nvfp4_dual_gemm_noalloc): fp32 partial slots followed by one ticket
@@ -90,7 +92,7 @@ struct DeviceState {
   bool ready = false;
   int num_sms = 0;
   unsigned* status = nullptr;
-  std::atomic<bool> smem_set[32] = {};  // one slot per kernel instantiation (any thread may set it)
+  std::atomic<bool> smem_set[64] = {};  // one slot per kernel instantiation (any thread may set it)
   int max_clusters[5] = {};  // co-resident clusters of the cluster split-K kernel, by size
   std::unordered_map<cudaStream_t, Workspace> ws;
   unsigned char* noalloc_scratch = nullptr;   // device address of g_noalloc_scratch
@@ -1197,4 +1199,321 @@ extern "C" int nvfp4_dual_gemm_noalloc(const void* a, const void* b1, const void
   if ((rc = noalloc_scratch(d, &al.fixed))) return rc;
   return run_dual(d, a, b1, b2, sfa, sfb1, sfb2, c, m, n, k, l, al,
                   static_cast<cudaStream_t>(stream_));
+}
+
+// ---------------------------------------------------------------------------
+// A few tokens times NVFP4 weights (plain, gated, per expert).
+// ---------------------------------------------------------------------------
+namespace nvfp4 {
+namespace {
+
+// Half of an SM's shared memory, less what a CTA has besides.
+constexpr int kGemvSmem = 112 * 1024;
+
+size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// Device workspace of a call: [groups (experts)][factors][images].
+struct GemvSpace { size_t back, image, total; };
+
+GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
+  const size_t k_blocks = (size_t)((k + kBK - 1) / kBK);
+  GemvSpace s;
+  s.back = moe ? align_up(sizeof(GemvGroups), 256) : 0;
+  s.image = align_up(s.back + (size_t)groups * kGemvTokens * kGemvMaxSplits * sizeof(float), 256);
+  s.total = s.image + k_blocks * ((size_t)rows * kGemvTokenBytes + (size_t)groups * kGemvXSfBytes);
+  return s;
+}
+
+// CTAs of a cluster that share a tile's K: the count (a power of two, so that
+// the 128 rows divide) with the fewest K blocks on the busiest CTA, when
+// `tiles` tiles go to one CTA per SM; the smaller count unless the larger saves
+// a tenth.
+int gemv_splits(long long tiles, int k_blocks, int num_sms) {
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= kGemvMaxSplits && s <= k_blocks; s *= 2) {
+    const long long clusters = num_sms / s;
+    const double load = (double)((tiles + clusters - 1) / clusters) * ((k_blocks + s - 1) / s);
+    if (s == 1 || load < 0.9 * least) best = s, least = load;
+  }
+  return best;
+}
+
+template <class Kern>
+int launch_chained(Kern kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
+                   const GemvParams& p, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (t_pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+template <bool kDual, bool kMoe, int kTmemCols>
+int launch_gemv(DeviceState* d, int slot, const GemvParams& p, int smem, long long tiles, cudaStream_t stream) {
+  auto kern = gemv_kernel<kDual, kMoe, kTmemCols>;
+  int rc = set_smem_once(d, slot, kern, kGemvSmem);
+  if (rc) return rc;
+  const int chunks = ((p.k_blocks + p.splits - 1) / p.splits + kExpandBlocks - 1) / kExpandBlocks;
+  const int rows = kMoe ? p.pairs : p.l * p.m;
+  rc = launch_chained(gemv_expand_kernel<kMoe>, dim3((unsigned)rows, (unsigned)(chunks * p.splits), 1), kExpandThreads, 0,
+                      1, stream, p, "gemv_expand_kernel");
+  if (rc) return rc;
+  const long long most = d->num_sms / p.splits;
+  const long long clusters = tiles < most ? tiles : most;
+  return launch_chained(kern, dim3((unsigned)(clusters * p.splits), 1, 1), kGemvThreads, smem, p.splits, stream, p,
+                        "gemv_kernel");
+}
+
+template <bool kDual, bool kMoe>
+int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream) {
+  const Knobs kn = read_knobs();
+  t_pdl = kn.pdl;
+  p.k_blocks = (p.k + kBK - 1) / kBK;
+  p.row_blocks = (p.n + kBM - 1) / kBM;
+  p.passes = (p.m + kGemvTokens - 1) / kGemvTokens;
+  const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
+  p.group_rows = rows < kGemvTokens ? rows : kGemvTokens;
+  const long long tiles = (long long)groups * p.row_blocks;
+  p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms);
+  while (p.splits > p.k_blocks) p.splits /= 2;
+  const GemvSpace sp = gemv_space(kMoe, kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  p.groups = reinterpret_cast<GemvGroups*>(ws);
+  p.back = reinterpret_cast<float*>(ws + sp.back);
+  p.image = ws + sp.image;
+  p.status = d->status;
+  p.wait_limit = wait_limit_cycles();
+  constexpr int kMats = kDual ? 2 : 1;
+  const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
+  const int sums = p.splits > 1 ? kMats * p.group_rows * kBM * (int)sizeof(float) : 0;
+  p.x_slots = x_bytes > 8192 ? 2 : kGemvMaxXSlots;
+  p.w_slots = (kGemvSmem - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
+  if (p.w_slots > kGemvMaxWSlots) p.w_slots = kGemvMaxWSlots;
+  const int smem = 1024 + p.w_slots * kGemvWBytes + p.x_slots * x_bytes + sums;
+  const int cols = kMats * ((p.group_rows * kGemvTerms + 15) / 16 * 16) + 16 * (p.w_slots + p.x_slots);
+  const int base = 32 + (kDual ? 4 : 0) + (kMoe ? 2 : 0);
+  if (cols <= 256) return launch_gemv<kDual, kMoe, 256>(d, base, p, smem, tiles, stream);
+  return launch_gemv<kDual, kMoe, 512>(d, base + 1, p, smem, tiles, stream);
+}
+
+int dtype_size(int t) { return t == kDtF32 ? 4 : 2; }
+bool dtype_ok(int t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
+
+// Sizes, types and alignment that all the products share.
+constexpr int kGemvMaxRows = 4096;   // rows of x in a batch entry
+
+int validate_gemv(const GemvParams& p, const void* workspace, size_t workspace_bytes, size_t need) {
+  if (!dtype_ok(p.x_dtype) || !dtype_ok(p.out_dtype)) return fail(NVFP4_ERR_INVALID_ARG, "bad dtype (x %d, out %d)", p.x_dtype, p.out_dtype);
+  if (p.k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", p.k);
+  if ((long long)p.n * p.k * p.l >= (1LL << 41) || (long long)p.m * p.l * p.k >= (1LL << 31))
+    return fail(NVFP4_ERR_SHAPE, "problem too large");
+  if (p.ldx < 0 || p.ldo < p.n) return fail(NVFP4_ERR_INVALID_ARG, "bad row strides (x %lld, out %lld)", (long long)p.ldx, (long long)p.ldo);
+  if (workspace_bytes < need) return fail(NVFP4_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+  if ((reinterpret_cast<uintptr_t>(p.x) & (dtype_size(p.x_dtype) - 1)) ||
+      (reinterpret_cast<uintptr_t>(p.out) & (dtype_size(p.out_dtype) - 1)) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(NVFP4_ERR_ALIGNMENT, "x and out must be aligned to their elements, the workspace to 256 bytes");
+  return NVFP4_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+extern "C" size_t nvfp4_gemv_workspace_bytes(int m, int k, int l) {
+  if (m < 1 || k < 1 || l < 1) return 0;
+  return gemv_space(false, (long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
+}
+
+extern "C" int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x_batch, const void* b1,
+                          const void* sf1, const void* b2, const void* sf2, void* out, int out_dtype,
+                          long long ldo, long long out_batch, int m, int n, int k, int l, void* workspace,
+                          size_t workspace_bytes, void* stream_) {
+  if (m < 0 || n < 1 || k < 1 || l < 1)
+    return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (m=%d n=%d k=%d l=%d)", m, n, k, l);
+  if (m == 0) return NVFP4_OK;
+  if (!x || !b1 || !sf1 || !out || !workspace || !b2 != !sf2) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if (m > kGemvMaxRows || l > 4096) return fail(NVFP4_ERR_SHAPE, "%d rows (at most %d), %d batch entries (at most 4096)", m, kGemvMaxRows, l);
+  if (!aligned16(b1) || !aligned16(b2) || !aligned16(sf1) || !aligned16(sf2))
+    return fail(NVFP4_ERR_ALIGNMENT, "weights and scale atoms must be 16-byte aligned");
+  GemvParams p = {};
+  p.sf1 = static_cast<const uint8_t*>(sf1), p.sf2 = static_cast<const uint8_t*>(sf2);
+  p.x = x, p.ldx = ldx, p.x_batch = x_batch, p.x_dtype = x_dtype;
+  p.out = out, p.out_dtype = out_dtype, p.ldo = ldo, p.out_batch = out_batch;
+  p.m = m, p.n = n, p.k = k, p.l = l;
+  int rc = validate_gemv(p, workspace, workspace_bytes, nvfp4_gemv_workspace_bytes(m, k, l));
+  if (rc) return rc;
+  const int es = dtype_size(x_dtype);
+  p.x_vec = aligned16(x) && ldx * es % 16 == 0 && x_batch * es % 16 == 0;
+  DeviceState* d = nullptr;
+  if ((rc = get_device(&d))) return rc;
+  if ((rc = encode_operand(&p.map1, b1, n, k, l, kBM))) return rc;
+  if (b2 && (rc = encode_operand(&p.map2, b2, n, k, l, kBM))) return rc;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  return b2 ? run_gemv<true, false>(d, p, workspace, stream) : run_gemv<false, false>(d, p, workspace, stream);
+}
+
+extern "C" size_t nvfp4_moe_table_bytes(int num_experts) {
+  return num_experts < 1 ? 0 : (size_t)num_experts * sizeof(GemvExpert);
+}
+
+extern "C" int nvfp4_moe_table(const void* const* b, const void* const* sfb_perm, int num_experts, int n, int k,
+                               void* table) {
+  if (num_experts < 1 || n < 1 || k < 1) return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (experts=%d n=%d k=%d)", num_experts, n, k);
+  if (!b || !sfb_perm || !table) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if (k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", k);
+  for (int e = 0; e < num_experts; ++e) {
+    if (!b[e] || !sfb_perm[e]) return fail(NVFP4_ERR_INVALID_ARG, "expert %d: null weights", e);
+    if (!aligned16(b[e]) || !aligned16(sfb_perm[e]))
+      return fail(NVFP4_ERR_ALIGNMENT, "expert %d: weights must be 16-byte aligned", e);
+  }
+  DeviceState* d = nullptr;
+  int rc = get_device(&d);
+  if (rc) return rc;
+  for (int e = 0; e < num_experts; ++e) {
+    GemvExpert entry;
+    memset(&entry, 0, sizeof(entry));
+    if ((rc = encode_operand_uncached(&entry.map, b[e], n, k, 1, kBM))) return rc;
+    entry.sf = static_cast<const uint8_t*>(sfb_perm[e]);
+    memcpy(static_cast<char*>(table) + (size_t)e * sizeof(GemvExpert), &entry, sizeof(entry));
+  }
+  return NVFP4_OK;
+}
+
+extern "C" size_t nvfp4_moe_gemv_workspace_bytes(int tokens, int topk, int k) {
+  if (tokens < 1 || topk < 1 || k < 1) return 0;
+  const long long pairs = (long long)tokens * topk;
+  return gemv_space(true, pairs, pairs, k).total;
+}
+
+extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_per_pair, const int* expert_ids,
+                              int tokens, int topk, const void* table1, const void* table2, int num_experts,
+                              void* out, int out_dtype, long long ldo, int n, int k, void* workspace,
+                              size_t workspace_bytes, void* stream_) {
+  if (tokens < 0 || topk < 1 || num_experts < 1 || n < 1 || k < 1)
+    return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (tokens=%d topk=%d experts=%d n=%d k=%d)", tokens, topk, num_experts, n, k);
+  if (tokens == 0) return NVFP4_OK;
+  if (!x || !expert_ids || !table1 || !out || !workspace) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if ((long long)tokens * topk > kGemvMaxPairs || num_experts > kGemvMaxExperts)
+    return fail(NVFP4_ERR_SHAPE, "%d x %d rows (at most %d; the dispatch and the grouped GEMM take more), %d experts (at most %d)",
+                tokens, topk, kGemvMaxPairs, num_experts, kGemvMaxExperts);
+  if ((reinterpret_cast<uintptr_t>(table1) & 63u) || (reinterpret_cast<uintptr_t>(table2) & 63u))
+    return fail(NVFP4_ERR_ALIGNMENT, "expert tables must be 64-byte aligned");
+  GemvParams p = {};
+  p.x = x, p.ldx = ldx, p.x_dtype = x_dtype;
+  p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
+  p.m = tokens, p.n = n, p.k = k, p.l = 1;
+  p.ids = expert_ids, p.pairs = tokens * topk, p.topk = topk, p.experts = num_experts;
+  p.x_per_pair = x_per_pair != 0;
+  p.table1 = static_cast<const GemvExpert*>(table1), p.table2 = static_cast<const GemvExpert*>(table2);
+  int rc = validate_gemv(p, workspace, workspace_bytes, nvfp4_moe_gemv_workspace_bytes(tokens, topk, k));
+  if (rc) return rc;
+  p.x_vec = aligned16(x) && ldx * dtype_size(x_dtype) % 16 == 0;
+  DeviceState* d = nullptr;
+  if ((rc = get_device(&d))) return rc;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  return table2 ? run_gemv<true, true>(d, p, workspace, stream) : run_gemv<false, true>(d, p, workspace, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Residual addition, root-mean-square norm and quantised output.
+// ---------------------------------------------------------------------------
+namespace nvfp4 {
+namespace {
+
+template <int NV, int kOut, bool kVec>
+int launch_norm_as(const NormParams& p, int threads, cudaStream_t stream) {
+  const int pad = kOut == kNormNvfp4 && p.rows % 128 ? (p.k / 64 + kNormPadAtoms - 1) / kNormPadAtoms : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.rows + pad), 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = t_pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm_kernel<NV, kOut, kVec>, p);
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "norm_kernel launch: %s", cudaGetErrorString(e));
+  return check_launch("norm_kernel");
+}
+
+template <int kOut, bool kVec>
+int launch_norm(DeviceState* d, const NormParams& p, cudaStream_t stream) {
+  const int chunks = (p.k + 7) / 8;
+  int nv = chunks <= kNormMaxThreads ? 1 : chunks <= 2 * kNormMaxThreads ? 2 : 4;
+  if (p.rows >= 2 * d->num_sms && chunks >= 4 * 32) nv = 4;
+  const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+  if (nv == 1) return launch_norm_as<1, kOut, kVec>(p, threads, stream);
+  if (nv == 2) return launch_norm_as<2, kOut, kVec>(p, threads, stream);
+  return launch_norm_as<4, kOut, kVec>(p, threads, stream);
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+extern "C" int nvfp4_rms_norm(const void* x, int x_dtype, long long ldx, const void* residual, int r_dtype,
+                              long long ldr, void* h, long long ldh, const void* weight, int w_dtype, double eps,
+                              int rows, int k, int format, void* y, int y_dtype, long long ldy, float* scales,
+                              int group, void* sf_perm, void* sf_plain, void* stream_) {
+  if (rows < 0 || k < 1) return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (rows=%d k=%d)", rows, k);
+  if (format < kNormPlain || format > kNormNvfp4) return fail(NVFP4_ERR_INVALID_ARG, "bad format %d", format);
+  if (!dtype_ok(x_dtype) || !dtype_ok(w_dtype) || (residual && !dtype_ok(r_dtype)) ||
+      (format == kNormPlain && !dtype_ok(y_dtype)))
+    return fail(NVFP4_ERR_INVALID_ARG, "bad dtype");
+  if (!(eps >= 0.0)) return fail(NVFP4_ERR_INVALID_ARG, "eps must not be negative");
+  if (k > kNormMaxK) return fail(NVFP4_ERR_SHAPE, "K=%d (at most %d)", k, kNormMaxK);
+  if (format == kNormNvfp4 && k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", k);
+  if (format == kNormFp8 && group != 0 && group != 32 && group != 64 && group != 128)
+    return fail(NVFP4_ERR_SHAPE, "group %d is none of 32, 64, 128 or 0 (the row)", group);
+  if (format == kNormFp8 && group != 0 && k % group != 0)
+    return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of the group (%d)", k, group);
+  if (rows == 0) return NVFP4_OK;
+  if (!x || !weight || !y || (residual && !h) || (format == kNormFp8 && !scales) || (format == kNormNvfp4 && !sf_perm))
+    return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if (ldx < 0 || (residual && (ldr < 0 || ldh < k)) || (format == kNormPlain && ldy < k))
+    return fail(NVFP4_ERR_INVALID_ARG, "bad row strides");
+  auto off = [](const void* q, int dtype) { return (reinterpret_cast<uintptr_t>(q) & (uintptr_t)(dtype_size(dtype) - 1)) != 0; };
+  if (off(x, x_dtype) || off(weight, w_dtype) || (residual && (off(residual, r_dtype) || off(h, r_dtype))) ||
+      (format == kNormPlain && off(y, y_dtype)) || (format == kNormFp8 && off(scales, kDtF32)))
+    return fail(NVFP4_ERR_ALIGNMENT, "tensors must be aligned to their elements");
+  if (format == kNormNvfp4 && (!aligned16(y) || !aligned16(sf_perm) || (reinterpret_cast<uintptr_t>(sf_plain) & 3u)))
+    return fail(NVFP4_ERR_ALIGNMENT, "packed and sf_perm need 16-byte, sf_plain 4-byte alignment");
+  DeviceState* d = nullptr;
+  int rc = get_device(&d);
+  if (rc) return rc;
+  const Knobs kn = read_knobs();
+  t_pdl = kn.pdl;
+  NormParams p = {};
+  p.x = x, p.residual = residual, p.weight = weight, p.h = residual ? h : nullptr;
+  p.ldx = ldx, p.ldr = ldr, p.ldh = ldh, p.eps = eps, p.rows = rows, p.k = k;
+  p.x_dtype = x_dtype, p.r_dtype = r_dtype, p.w_dtype = w_dtype;
+  p.y = y, p.ldy = ldy, p.y_dtype = y_dtype, p.scales = scales, p.group = group;
+  p.sf_perm = static_cast<uint8_t*>(sf_perm), p.sf_plain = static_cast<uint8_t*>(sf_plain);
+  auto lines = [](const void* q, int dtype, long long ld) { return aligned16(q) && ld * dtype_size(dtype) % 16 == 0; };
+  const bool vec = k % 8 == 0 && lines(x, x_dtype, ldx) && lines(weight, w_dtype, 0) &&
+                   (!residual || (lines(residual, r_dtype, ldr) && lines(h, r_dtype, ldh))) &&
+                   (format == kNormPlain ? lines(y, y_dtype, ldy) : (reinterpret_cast<uintptr_t>(y) & 7u) == 0);
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (format == kNormPlain) return vec ? launch_norm<kNormPlain, true>(d, p, stream) : launch_norm<kNormPlain, false>(d, p, stream);
+  if (format == kNormFp8) return vec ? launch_norm<kNormFp8, true>(d, p, stream) : launch_norm<kNormFp8, false>(d, p, stream);
+  return vec ? launch_norm<kNormNvfp4, true>(d, p, stream) : launch_norm<kNormNvfp4, false>(d, p, stream);
 }

@@ -1,0 +1,349 @@
+// Residual addition, root-mean-square norm and quantised output, sm_100a:
+//
+//   h = rn(x + residual)                    (rounded to the residual's type; h = x without one)
+//   r = rn(1 / sqrt(sum(h^2) / K + eps))    (the sum and the root in fp64, r in fp32)
+//   y = rn(rn(h * r) * weight)              (fp32)
+//
+// and y as
+//   kNormPlain  fp16, bf16 or fp32;
+//   kNormFp8    e4m3 with one fp32 scale for each `group` columns (or the whole
+//               row): s = amax / 448, q = e4m3_rne(y / s), all zero when s is 0;
+//   kNormNvfp4  e2m1 + e4m3 scales per 16 in the layouts the GEMMs read, by the
+//               rules of quantize.cuh.
+//
+// The sum is fp64 because it decides on which side of a rounding border a
+// code falls: summed in fp32 the last bit of r depends on the order of the
+// sum, and codes on a border move with it.  In fp64 two orders differ by
+// about 2^-53, so that r, and with it every output bit, is the same for any
+// number of threads (but for one row in about 2^28).
+//
+// A row is read once: each thread keeps its elements in registers from the
+// load to the output.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cstdint>
+#include "gemv.cuh"
+#include "ptx.cuh"
+#include "quantize.cuh"
+
+namespace nvfp4 {
+
+constexpr int kNormPlain = 0, kNormFp8 = 1, kNormNvfp4 = 2;
+constexpr int kNormMaxThreads = 1024;
+constexpr int kNormMaxK = kNormMaxThreads * 8 * 4;
+constexpr int kNormPadAtoms = 8;       // scale atoms whose padding rows one CTA clears
+
+struct NormParams {
+  const void *x, *residual, *weight;   // residual may be null
+  void* h;                             // [rows][k], the residual's type; null without a residual
+  int64_t ldx, ldr, ldh;
+  double eps;
+  int rows, k, x_dtype, r_dtype, w_dtype;
+  void* y;                             // plain: [rows][k]; fp8: e4m3 bytes; nvfp4: packed [rows][k/2]
+  int64_t ldy;                         // plain only
+  int y_dtype;                         // plain only
+  float* scales;                       // fp8: [rows][k / group]
+  int group;                           // fp8: 32, 64 or 128 columns, 0 for the row
+  uint8_t *sf_perm, *sf_plain;         // nvfp4
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct Raw8 { uint4 a, b; };           // eight elements as they lie in memory (b: fp32 only)
+
+template <bool kVec>
+__device__ __forceinline__ Raw8 norm_load8(const void* base, int dtype, int64_t at, int left) {
+  Raw8 r;
+  r.a = r.b = make_uint4(0, 0, 0, 0);
+  if (left <= 0) return r;
+  if (dtype == kDtF32) {
+    const uint32_t* q = static_cast<const uint32_t*>(base) + at;
+    if constexpr (kVec) {
+      r.a = *reinterpret_cast<const uint4*>(q), r.b = *reinterpret_cast<const uint4*>(q + 4);
+    } else {
+      uint32_t v[8];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < left ? q[i] : 0u;
+      r.a = make_uint4(v[0], v[1], v[2], v[3]), r.b = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(base) + at;
+    if constexpr (kVec) {
+      r.a = *reinterpret_cast<const uint4*>(q);
+    } else {
+      uint32_t v[4];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = (2 * i < left ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+      r.a = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ void norm_widen(const Raw8& r, int dtype, float (&f)[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if (dtype == kDtF32) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+  } else if (dtype == kDtBF16) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x, f[2 * i + 1] = t.y;
+    }
+  }
+}
+
+// fp32 -> the type's bits; `f` becomes the rounded values.
+__device__ __forceinline__ Raw8 norm_round(float (&f)[8], int dtype) {
+  Raw8 r;
+  uint32_t w[8];
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
+  if (dtype == kDtF32) {
+    r.a = make_uint4(w[0], w[1], w[2], w[3]), r.b = make_uint4(w[4], w[5], w[6], w[7]);
+    return r;
+  }
+  uint32_t h[4];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dtype == kDtBF16) {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      h[i] = *reinterpret_cast<const uint32_t*>(&t);
+    } else {
+      const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      h[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  r.a = make_uint4(h[0], h[1], h[2], h[3]), r.b = make_uint4(0, 0, 0, 0);
+  norm_widen(r, dtype, f);
+  return r;
+}
+
+template <bool kVec>
+__device__ __forceinline__ void norm_store8(void* base, int dtype, int64_t at, int left, const Raw8& r) {
+  if (left <= 0) return;
+  if (dtype == kDtF32) {
+    uint32_t* q = static_cast<uint32_t*>(base) + at;
+    if constexpr (kVec) {
+      *reinterpret_cast<uint4*>(q) = r.a, *reinterpret_cast<uint4*>(q + 4) = r.b;
+    } else {
+      const uint32_t v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+      #pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) q[i] = v[i];
+    }
+  } else {
+    uint16_t* q = static_cast<uint16_t*>(base) + at;
+    if constexpr (kVec) {
+      *reinterpret_cast<uint4*>(q) = r.a;
+    } else {
+      const uint32_t v[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+      #pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) q[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// RN(y / s) for a whole group: by the two fused multiply-adds of
+// quantize.cuh's div_by_scale where Markstein's theorem holds (r = RN(1 / s),
+// s's mantissa not all ones, nothing near under- or overflow), else by the
+// division itself.
+__device__ __forceinline__ bool norm_fast_scale(float s) {
+  return s >= 8.077936e-28f /* 2^-90 */ && s <= 1.329228e36f /* 2^120 */ &&
+         (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu;
+}
+
+// One CTA for each row (chunks of 8 elements, chunk c = thread + i * threads,
+// i < NV); kNormNvfp4: CTAs past the rows clear the padding rows of the last
+// block's scale atoms.  kVec: every 8 elements of every tensor are 16-byte aligned
+// and K % 8 == 0.
+template <int NV, int kOut, bool kVec>
+__global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __grid_constant__ NormParams p) {
+  __shared__ double s_sum[32];
+  __shared__ float s_max[32];
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+  griddep_wait();
+  griddep_launch_dependents();
+  if constexpr (kOut == kNormNvfp4) {
+    if ((int)blockIdx.x >= p.rows) {
+      const int rest = p.rows % 128, atoms = p.k / 64;
+      const int a0 = ((int)blockIdx.x - p.rows) * kNormPadAtoms, a1 = min(a0 + kNormPadAtoms, atoms);
+      uint32_t* base = reinterpret_cast<uint32_t*>(p.sf_perm + (size_t)(p.rows / 128) * atoms * 512);
+      for (int i = a0 * 128 + tid; i < a1 * 128; i += (int)blockDim.x) {
+        const int w = i % 128;                            // word of the atom: row w/4 of quarter w%4
+        if ((w % 4) * 32 + w / 4 >= rest) base[i] = 0u;
+      }
+      return;
+    }
+  }
+  const int row = (int)blockIdx.x;
+  float v[NV][8];
+  Raw8 wt[NV];
+  #pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (tid + i * (int)blockDim.x) * 8;
+    const Raw8 rx = norm_load8<kVec>(p.x, p.x_dtype, (int64_t)row * p.ldx + col, p.k - col);
+    norm_widen(rx, p.x_dtype, v[i]);
+    wt[i] = norm_load8<kVec>(p.weight, p.w_dtype, col, p.k - col);
+  }
+  if (p.residual != nullptr) {
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (tid + i * (int)blockDim.x) * 8;
+      const Raw8 rr = norm_load8<kVec>(p.residual, p.r_dtype, (int64_t)row * p.ldr + col, p.k - col);
+      float f[8];
+      norm_widen(rr, p.r_dtype, f);
+      #pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(v[i][e], f[e]);
+      const Raw8 h = norm_round(v[i], p.r_dtype);
+      norm_store8<kVec>(p.h, p.r_dtype, (int64_t)row * p.ldh + col, p.k - col, h);
+    }
+  }
+  double sum = 0.0;
+  #pragma unroll
+  for (int i = 0; i < NV; ++i)
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double d = (double)v[i][e];
+      sum = fma(d, d, sum);
+    }
+  #pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (warps > 1) {
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = lane < warps ? s_sum[lane] : 0.0;
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  const float r = (float)(1.0 / sqrt(sum / p.k + p.eps));
+  #pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float w[8];
+    norm_widen(wt[i], p.w_dtype, w);
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], r), w[e]);
+  }
+
+  if constexpr (kOut == kNormPlain) {
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (tid + i * (int)blockDim.x) * 8;
+      norm_store8<kVec>(p.y, p.y_dtype, (int64_t)row * p.ldy + col, p.k - col, norm_round(v[i], p.y_dtype));
+    }
+  } else if constexpr (kOut == kNormFp8) {
+    float top[NV];
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      // chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then
+      top[i] = 0.f;
+      #pragma unroll
+      for (int e = 0; e < 8; ++e) top[i] = max_nan(top[i], fabsf(v[i][e]));
+    }
+    if (p.group == 0) {
+      float m = top[0];
+      #pragma unroll
+      for (int i = 1; i < NV; ++i) m = max_nan(m, top[i]);
+      #pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (warps > 1) {
+        if (lane == 0) s_max[warp] = m;
+        __syncthreads();
+        m = lane < warps ? s_max[lane] : 0.f;
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
+      #pragma unroll
+      for (int i = 0; i < NV; ++i) top[i] = m;
+    } else {
+      const int lanes = p.group / 8;                      // 4, 8 or 16 neighbouring lanes
+      #pragma unroll
+      for (int i = 0; i < NV; ++i)
+        for (int o = 1; o < lanes; o <<= 1) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+    }
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (tid + i * (int)blockDim.x) * 8;
+      const int left = p.k - col;
+      const float s = __fdiv_rn(top[i], 448.f);
+      uint32_t code[2] = {0u, 0u};
+      if (s != 0.f) {
+        const bool fast = norm_fast_scale(s);
+        const float rs = fast ? __frcp_rn(s) : 0.f;
+        #pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float q0 = fast ? div_by_scale(v[i][e], s, rs) : __fdiv_rn(v[i][e], s);
+          const float q1 = fast ? div_by_scale(v[i][e + 1], s, rs) : __fdiv_rn(v[i][e + 1], s);
+          const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3);
+          code[e / 4] |= two << (8 * (e % 4));
+        }
+      }
+      if (left > 0) {
+        uint8_t* q = static_cast<uint8_t*>(p.y) + (int64_t)row * p.k + col;
+        if constexpr (kVec) {
+          *reinterpret_cast<uint2*>(q) = make_uint2(code[0], code[1]);
+        } else {
+          #pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) q[e] = (uint8_t)(code[e / 4] >> (8 * (e % 4)));
+        }
+        if (p.group == 0) {
+          if (tid == 0 && i == 0) p.scales[row] = s;
+        } else if (col % p.group == 0) {
+          p.scales[(int64_t)row * (p.k / p.group) + col / p.group] = s;
+        }
+      }
+    }
+  } else {
+    const int sub = lane & 7;                             // chunk of the 64-column atom
+    #pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (tid + i * (int)blockDim.x) * 8;
+      float amax = 0.f;
+      #pragma unroll
+      for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(v[i][e]));
+      amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      const bool finite = amax <= 3.402823466e38f;
+      const float a6 = finite ? div_by_scale(amax, 6.0f, 1.0f / 6.0f) : amax;
+      const __nv_fp8_storage_t s8 = __nv_cvt_float_to_fp8(a6, __NV_SATFINITE, __NV_E4M3);
+      const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(s8, __NV_E4M3)));
+      uint32_t word = 0;
+      if (s != 0.f) {
+        const float rs = __frcp_rn(s);
+        #pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float q0 = finite ? div_by_scale(v[i][e], s, rs) : __fdiv_rn(v[i][e], s);
+          const float q1 = finite ? div_by_scale(v[i][e + 1], s, rs) : __fdiv_rn(v[i][e + 1], s);
+          word |= e2m1x2(q0, q1) << (4 * e);
+        }
+      }
+      const uint32_t pair = (uint32_t)s8 | (__shfl_down_sync(0xffffffffu, (uint32_t)s8, 2) << 8);
+      const uint32_t sf_word = pair | (__shfl_down_sync(0xffffffffu, pair, 4) << 16);   // sub 0
+      if (col < p.k) {
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + (int64_t)row * (p.k / 2) + col / 2) = word;
+        if (sub == 0) {
+          const int atom = col / 64;
+          *reinterpret_cast<uint32_t*>(p.sf_perm + ((size_t)(row / 128) * (p.k / 64) + atom) * 512 + (row % 32) * 16 +
+                                       (row % 128 / 32) * 4) = sf_word;
+          if (p.sf_plain != nullptr)
+            *reinterpret_cast<uint32_t*>(p.sf_plain + (int64_t)row * (p.k / 16) + atom * 4) = sf_word;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace nvfp4

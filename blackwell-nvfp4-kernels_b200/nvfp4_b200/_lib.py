@@ -19,6 +19,14 @@ NVFP4_ERR_CUDA = -4
 NVFP4_ERR_DEVICE = -5
 NVFP4_ERR_TIMEOUT = -6
 
+# element types of the calls that take several, and the norm's outputs
+NVFP4_F32 = 0
+NVFP4_F16 = 1
+NVFP4_BF16 = 2
+NVFP4_NORM_PLAIN = 0
+NVFP4_NORM_FP8 = 1
+NVFP4_NORM_NVFP4 = 2
+
 # every symbol include/nvfp4_b200.h declares
 EXPORTED = (
     "nvfp4_dual_gemm",
@@ -30,6 +38,13 @@ EXPORTED = (
     "nvfp4_moe_sf_bytes",
     "nvfp4_moe_combine",
     "nvfp4_moe_grouped_gemm",
+    "nvfp4_gemv",
+    "nvfp4_gemv_workspace_bytes",
+    "nvfp4_moe_table",
+    "nvfp4_moe_table_bytes",
+    "nvfp4_moe_gemv",
+    "nvfp4_moe_gemv_workspace_bytes",
+    "nvfp4_rms_norm",
     "nvfp4_device_status",
     "nvfp4_wait_selftest",
     "nvfp4_status_string",
@@ -96,6 +111,24 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     pp = ctypes.POINTER(ctypes.c_void_p)
     lib.nvfp4_moe_grouped_gemm.argtypes = [vp, i32, vp, vp, vp, vp, pp, pp, i32, i32, i32, vp, vp]
     lib.nvfp4_moe_grouped_gemm.restype = i32
+    i64 = ctypes.c_longlong
+    lib.nvfp4_gemv.argtypes = [vp, i32, i64, i64, vp, vp, vp, vp, vp, i32, i64, i64, i32, i32, i32, i32,
+                               vp, sz, vp]
+    lib.nvfp4_gemv.restype = i32
+    lib.nvfp4_gemv_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.nvfp4_gemv_workspace_bytes.restype = sz
+    lib.nvfp4_moe_gemv.argtypes = [vp, i32, i64, i32, vp, i32, i32, vp, vp, i32, vp, i32, i64, i32, i32,
+                                   vp, sz, vp]
+    lib.nvfp4_moe_gemv.restype = i32
+    lib.nvfp4_moe_gemv_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.nvfp4_moe_gemv_workspace_bytes.restype = sz
+    lib.nvfp4_moe_table.argtypes = [pp, pp, i32, i32, i32, vp]
+    lib.nvfp4_moe_table.restype = i32
+    lib.nvfp4_moe_table_bytes.argtypes = [i32]
+    lib.nvfp4_moe_table_bytes.restype = sz
+    lib.nvfp4_rms_norm.argtypes = [vp, i32, i64, vp, i32, i64, vp, i64, vp, i32, ctypes.c_double, i32, i32,
+                                   i32, vp, i32, i64, vp, i32, vp, vp, vp]
+    lib.nvfp4_rms_norm.restype = i32
     lib.nvfp4_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint)]
     lib.nvfp4_device_status.restype = i32
     lib.nvfp4_wait_selftest.argtypes = [ctypes.c_longlong, vp]

@@ -18,7 +18,8 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libnvfp4_b200.so"
 SOURCES = ["capi.cu"]
 HEADERS = ["ptx.cuh", "kernel_common.cuh", "dual_gemm.cuh", "dual_gemm_2sm.cuh", "grouped_gemm_2sm.cuh",
-           "grouped_gemm.cuh", "quantize.cuh", "moe.cuh"]
+           "grouped_gemm.cuh", "quantize.cuh", "moe.cuh", "gemv.cuh",
+           "norm.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

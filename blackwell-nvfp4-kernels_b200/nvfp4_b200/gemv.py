@@ -1,0 +1,111 @@
+"""A few tokens times NVFP4 weights (``nvfp4_gemv`` in libnvfp4_b200.so).
+
+The GEMMs of this package quantise the activations and work on 128-row tiles.
+For the one to sixteen tokens of a decoding step these products read the same
+weights in the same layout (``quantize.quantize``, ``formats``) once, and take the
+activations as they are, fp16, bf16 or fp32, with fp32 sums:
+
+    w1, w2 = gemv.Weights(b1, sfb1_perm), gemv.Weights(b2, sfb2_perm)
+    h = gemv.dual_gemv(x, w1, w2)        # silu(x . W1ᵀ) * (x . W2ᵀ)
+    y = gemv.gemv(h, w3)                 # h . W3ᵀ
+
+The per-expert forms are ``moe.gemv`` and ``moe.dual_gemv``.  Counterparts in the
+reference: the dual and the grouped GEMM (nvfp4_dual_gemm/reference.py:27-77,
+nvfp4_group_gemm/reference.py:39-74), which take quantised activations.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .dual_gemm import check_sf_perm, on_device
+from .formats import ceil_div
+
+DTYPES = {torch.float32: _lib.NVFP4_F32, torch.float16: _lib.NVFP4_F16,
+          torch.bfloat16: _lib.NVFP4_BF16}
+
+
+class Weights:
+    """One NVFP4 weight matrix (or L of them), checked once.
+
+    ``b``: float4_e2m1fn_x2 (or uint8) [N, K/2] or [N, K/2, L], K-major, batch
+    outermost; ``sfb_perm``: its permuted scales, float8_e4m3fn (or uint8)
+    [32, 4, ceil(N/128), 4, K/64, L], or that tensor's memory, contiguous
+    [(L,) ceil(N/128), K/64, 32, 4, 4].  K % 64 == 0.  The tensors are kept."""
+
+    def __init__(self, b: torch.Tensor, sfb_perm: torch.Tensor):
+        if not b.is_cuda or b.dim() not in (2, 3):
+            raise ValueError("b must be a CUDA tensor [N, K/2] or [N, K/2, L]")
+        if b.dtype not in (torch.float4_e2m1fn_x2, torch.uint8, torch.int8):
+            raise ValueError(f"b: expected float4_e2m1fn_x2, got {b.dtype}")
+        n, kh = int(b.shape[0]), int(b.shape[1])
+        l = int(b.shape[2]) if b.dim() == 3 else 1
+        k = 2 * kh
+        if n < 1 or l < 1 or k < 64 or k % 64:
+            raise ValueError(f"b: N={n}, L={l} must be positive and K={k} a positive multiple of 64")
+        if b.stride(1) != 1 or (n > 1 and b.stride(0) != kh) or (l > 1 and b.stride(2) != n * kh):
+            raise ValueError(f"b: strides {b.stride()} are not the K-major [L][{n}][{kh}] layout")
+        if sfb_perm.dim() == 6 and tuple(sfb_perm.shape[:2]) == (32, 4):
+            check_sf_perm("sfb_perm", sfb_perm, n, k, l, b.device)
+        else:
+            atoms = (ceil_div(n, 128), k // 64, 32, 4, 4)
+            if tuple(sfb_perm.shape) not in ((l,) + atoms, *((atoms,) if l == 1 else ())):
+                raise ValueError(f"sfb_perm: shape {tuple(sfb_perm.shape)} holds no scales of [{n}, {k}, {l}]")
+            if sfb_perm.dtype not in (torch.float8_e4m3fn, torch.uint8, torch.int8):
+                raise ValueError(f"sfb_perm: expected float8_e4m3fn, got {sfb_perm.dtype}")
+            if not sfb_perm.is_contiguous() or sfb_perm.device != b.device:
+                raise ValueError(f"sfb_perm must be contiguous on {b.device}")
+        self.b, self.sfb_perm = b, sfb_perm
+        self.n, self.k, self.l, self.device = n, k, l, b.device
+        self.ptrs = (b.data_ptr(), sfb_perm.data_ptr())
+
+
+def _rows_last(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _run(x, w, w2, out, out_dtype):
+    if x.dim() not in (2, 3) or x.dtype not in DTYPES:
+        raise ValueError("x must be float16, bfloat16 or float32 [M, K] or [L, M, K]")
+    if x.device != w.device:
+        raise ValueError(f"x is on {x.device}, the weights on {w.device}")
+    batched = x.dim() == 3
+    if x.shape[-1] != w.k or (x.shape[0] if batched else 1) != w.l:
+        raise ValueError(f"x {tuple(x.shape)} does not match weights of K={w.k}, L={w.l}")
+    m = int(x.shape[-2])
+    x = _rows_last(x)
+    shape = (w.l, m, w.n) if batched else (m, w.n)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=x.device)
+    elif (tuple(out.shape) != shape or out.dtype not in DTYPES or out.device != x.device
+          or out.dtype != (out_dtype or out.dtype) or (out.stride(-1) != 1 and w.n > 1)
+          or (m > 1 and out.stride(-2) < w.n)
+          or (batched and w.l > 1 and out.stride(0) < (m - 1) * out.stride(1) + w.n)):
+        raise ValueError(f"out must be {shape}, float16, bfloat16 or float32, rows apart, on {x.device}")
+    lib = _lib.load()
+    b2 = w2.ptrs if w2 is not None else (None, None)
+    size = lib.nvfp4_gemv_workspace_bytes(m, w.k, w.l)
+    space = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _lib.check(on_device(x.device, lambda st: lib.nvfp4_gemv(
+        x.data_ptr(), DTYPES[x.dtype], x.stride(-2), x.stride(0) if batched else 0, *w.ptrs, *b2,
+        out.data_ptr(), DTYPES[out.dtype], max(out.stride(-2), w.n), out.stride(0) if batched else 0,
+        m, w.n, w.k, w.l, space.data_ptr(), size, st)))
+    return out
+
+
+def gemv(x: torch.Tensor, w: Weights, out: torch.Tensor | None = None,
+         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x . Wᵀ for x [M, K] (or [L, M, K], L matrices): [M, N] (or [L, M, N]) in
+    ``out_dtype`` (x's type by default; fp16, bf16 or fp32), one rounding of an
+    fp32 sum.  ``out``: written and returned instead of a new tensor; its rows may
+    be strided.  Meant for M <= 16; every 16 further tokens (8 in fp32) read the
+    weights again."""
+    return _run(x, w, None, out, out_dtype)
+
+
+def dual_gemv(x: torch.Tensor, w1: Weights, w2: Weights, out: torch.Tensor | None = None,
+              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """silu(x . W1ᵀ) * (x . W2ᵀ), the gate in fp32; otherwise as :func:`gemv`."""
+    if (w1.n, w1.k, w1.l, w1.device) != (w2.n, w2.k, w2.l, w2.device):
+        raise ValueError("w1 and w2 must have the same N, K, L and device")
+    return _run(x, w1, w2, out, out_dtype)

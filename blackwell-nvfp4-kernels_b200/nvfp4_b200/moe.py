@@ -21,6 +21,7 @@ import torch
 
 from . import _lib
 from .dual_gemm import on_device
+from .gemv import DTYPES, _rows_last
 
 
 @dataclass
@@ -150,6 +151,19 @@ class ExpertWeights:
                 raise ValueError(f"expert {i}: scales must hold {rn * rk * 512} bytes on {b0.device}")
         self.b_ptrs = arr(*[b.data_ptr() for b, _ in self.w])
         self.sfb_ptrs = arr(*[s.data_ptr() for _, s in self.w])
+        self.device = b0.device
+        self._table = None
+
+    def table(self) -> torch.Tensor:
+        """The experts' weights as :func:`gemv` finds them in device memory (made by
+        the first call that needs it)."""
+        if self._table is None:
+            lib = _lib.load()
+            host = (ctypes.c_char * int(lib.nvfp4_moe_table_bytes(len(self.w))))()
+            with torch.cuda.device(self.device):
+                _lib.check(lib.nvfp4_moe_table(self.b_ptrs, self.sfb_ptrs, len(self.w), self.n, self.k, host))
+                self._table = torch.frombuffer(host, dtype=torch.uint8).to(self.device)
+        return self._table
 
     def __len__(self):
         return len(self.w)
@@ -197,3 +211,67 @@ def combine(c_all: torch.Tensor, d: Dispatch, weights: torch.Tensor | None = Non
         weights.data_ptr() if weights is not None else None,
         d.tokens, d.topk, n, out.data_ptr(), st)))
     return out
+
+
+def _products(x, expert_ids, w, w2, out, out_dtype):
+    ids = expert_ids if expert_ids.dim() == 2 else expert_ids.unsqueeze(1)
+    if ids.dim() != 2 or ids.dtype != torch.int32:
+        raise ValueError("expert_ids must be int32 [tokens] or [tokens, topk]")
+    if x.dim() != 2 or x.dtype not in DTYPES:
+        raise ValueError("x must be float16, bfloat16 or float32 [tokens or tokens*topk, K]")
+    if not (x.device == ids.device == w.device):
+        raise ValueError(f"x, expert_ids and the weights must be on one device ({w.device})")
+    tokens, topk = ids.shape
+    rows = tokens * topk
+    if x.shape[1] != w.k or x.shape[0] not in (tokens, rows):
+        raise ValueError(f"x {tuple(x.shape)} is neither [{tokens}, {w.k}] nor [{rows}, {w.k}]")
+    x, ids = _rows_last(x), ids.contiguous()
+    if out is None:
+        out = torch.empty((rows, w.n), dtype=out_dtype or x.dtype, device=x.device)
+    elif (tuple(out.shape) != (rows, w.n) or out.dtype not in DTYPES or out.device != x.device
+          or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and w.n > 1)
+          or (rows > 1 and out.stride(0) < w.n)):
+        raise ValueError(f"out must be [{rows}, {w.n}], float16, bfloat16 or float32, rows apart, on {x.device}")
+    lib = _lib.load()
+    size = lib.nvfp4_moe_gemv_workspace_bytes(tokens, topk, w.k)
+    space = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _lib.check(on_device(x.device, lambda st: lib.nvfp4_moe_gemv(
+        x.data_ptr(), DTYPES[x.dtype], x.stride(0), int(x.shape[0] == rows and topk > 1), ids.data_ptr(),
+        tokens, topk, w.table().data_ptr(), w2.table().data_ptr() if w2 is not None else None, len(w),
+        out.data_ptr(), DTYPES[out.dtype], max(out.stride(0), w.n), w.n, w.k, space.data_ptr(), size, st)))
+    return out
+
+
+def gemv(x: torch.Tensor, expert_ids: torch.Tensor, weights: ExpertWeights,
+         out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Row t*topk + j of the result is x_row . W_eᵀ with e = expert_ids[t, j] (int32
+    [T] or [T, topk]): a decoding step's experts without a dispatch, activations not
+    quantised, each chosen expert's weights read once for every 16 of its rows.
+    ``x``: float16, bfloat16 or float32, [T, K] (token t's row for all its choices)
+    or [T*topk, K] (a row for each choice).  A row whose id is outside
+    [0, experts) is zero.  Result [T*topk, N] in ``out_dtype`` (x's type by
+    default); float16 goes into :func:`combine` with :func:`pair_order`.  At most
+    256 rows: ``dispatch`` and ``grouped_gemm`` are for more."""
+    return _products(x, expert_ids, weights, None, out, out_dtype)
+
+
+def dual_gemv(x: torch.Tensor, expert_ids: torch.Tensor, w1: ExpertWeights, w2: ExpertWeights,
+              out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """silu(x_row . W1_eᵀ) * (x_row . W2_eᵀ) for each choice; otherwise as :func:`gemv`."""
+    if (len(w1), w1.n, w1.k, w1.device) != (len(w2), w2.n, w2.k, w2.device):
+        raise ValueError("w1 and w2 must have the same number of experts, N, K and device")
+    return _products(x, expert_ids, w1, w2, out, out_dtype)
+
+
+@dataclass
+class PairOrder:
+    """Rows in the order of the choices (row t*topk + j), as :func:`gemv` leaves
+    them: stands in for a Dispatch in :func:`combine`."""
+    dst: torch.Tensor
+    tokens: int
+    topk: int
+
+
+def pair_order(tokens: int, topk: int, device) -> PairOrder:
+    """Made once for each (tokens, topk)."""
+    return PairOrder(torch.arange(tokens * topk, dtype=torch.int32, device=device), tokens, topk)

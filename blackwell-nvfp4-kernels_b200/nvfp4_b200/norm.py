@@ -1,0 +1,135 @@
+"""Residual addition, root-mean-square norm and quantised output in one pass
+(``nvfp4_rms_norm`` in libnvfp4_b200.so): what stands before the projections of a block.
+
+    h = x + residual                     (rounded to the residual's type)
+    y = h / sqrt(mean(h^2) + eps) * weight
+
+:func:`rms_norm` returns y in 16 or 32 bits (the input of ``gemv``),
+:func:`rms_norm_fp8` in e4m3 with fp32 scales, :func:`rms_norm_nvfp4` in the
+layouts of ``quantize.quantize`` (the A operand of the GEMMs).  Each returns
+``(y, h)``; h is the residual of the next block, x itself where no residual is given.
+The reference takes its operands quantised (nvfp4_dual_gemm/reference.py:113-187)
+and has no counterpart.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .dual_gemm import on_device
+from .gemv import DTYPES, _rows_last
+
+
+def _check(x, weight, residual, residual_out):
+    """(x, weight, residual, h): checked, rows with unit stride."""
+    if x.dim() != 2 or x.dtype not in DTYPES or not x.is_cuda:
+        raise ValueError("x must be a CUDA float16, bfloat16 or float32 tensor [rows, K]")
+    rows, k = x.shape
+    if tuple(weight.shape) != (k,) or weight.dtype not in DTYPES or weight.device != x.device:
+        raise ValueError(f"weight must be float16, bfloat16 or float32 [{k}] on {x.device}")
+    if k < 1:
+        raise ValueError("K must be positive")
+    x, weight = _rows_last(x), weight.contiguous()
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError("residual_out without a residual")
+        return x, weight, None, None
+    if tuple(residual.shape) != (rows, k) or residual.dtype not in DTYPES or residual.device != x.device:
+        raise ValueError(f"residual must be float16, bfloat16 or float32 [{rows}, {k}] on {x.device}")
+    h = residual_out
+    if h is None:
+        h = torch.empty((rows, k), dtype=residual.dtype, device=x.device)
+    elif (tuple(h.shape) != (rows, k) or h.dtype != residual.dtype or h.device != x.device
+          or (h.stride(1) != 1 and k > 1) or (rows > 1 and h.stride(0) < k)):
+        raise ValueError(f"residual_out must be {residual.dtype} [{rows}, {k}], rows apart, on {x.device}")
+    return x, weight, _rows_last(residual), h
+
+
+def _run(x, weight, residual, h, eps, fmt, y, y_dtype=0, ldy=0, scales=None, group=0, sf_perm=None, sf=None):
+    lib = _lib.load()
+    rows, k = x.shape
+    _lib.check(on_device(x.device, lambda st: lib.nvfp4_rms_norm(
+        x.data_ptr(), DTYPES[x.dtype], x.stride(0),
+        *((residual.data_ptr(), DTYPES[residual.dtype], residual.stride(0), h.data_ptr(), max(h.stride(0), k))
+          if residual is not None else (None, 0, 0, None, 0)),
+        weight.data_ptr(), DTYPES[weight.dtype], eps, rows, k, fmt, y, y_dtype, ldy, scales, group, sf_perm, sf,
+        st)))
+    return x if residual is None else h
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+             eps: float = 1e-6, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+             residual_out: torch.Tensor | None = None):
+    """(y, h) for x [rows, K], K <= 32768; y [rows, K] in ``out_dtype`` (x's type by
+    default).  x, weight, residual and y may each be float16, bfloat16 or float32;
+    ``residual_out`` may be ``residual`` itself (then updated in place)."""
+    x, weight, residual, h = _check(x, weight, residual, residual_out)
+    rows, k = x.shape
+    if out is None:
+        out = torch.empty((rows, k), dtype=out_dtype or x.dtype, device=x.device)
+    elif (tuple(out.shape) != (rows, k) or out.dtype not in DTYPES or out.device != x.device
+          or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and k > 1)
+          or (rows > 1 and out.stride(0) < k)):
+        raise ValueError(f"out must be [{rows}, {k}], float16, bfloat16 or float32, rows apart, on {x.device}")
+    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_PLAIN, out.data_ptr(), DTYPES[out.dtype],
+             max(out.stride(0), k))
+    return out, h
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+                 eps: float = 1e-6, group: int | None = 128, out=None,
+                 residual_out: torch.Tensor | None = None):
+    """((q, scales), h): q float8_e4m3fn [rows, K] and scales float32 [rows, K/group]
+    with y = q * scale; scale = amax/448 over ``group`` columns (32, 64 or 128,
+    dividing K; None: the row), q = e4m3(y / scale) to nearest even, zeros under a
+    zero scale; a NaN gives its group a NaN scale.  ``out``: the (q, scales) of an
+    earlier call of the same sizes, reused."""
+    x, weight, residual, h = _check(x, weight, residual, residual_out)
+    rows, k = x.shape
+    if group not in (None, 32, 64, 128):
+        raise ValueError(f"group {group} is none of 32, 64, 128 or None (the row)")
+    if group is not None and k % group:
+        raise ValueError(f"K={k} must be a multiple of the group ({group})")
+    groups = 1 if group is None else k // group
+    if out is None:
+        q = torch.empty((rows, k), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((rows, groups), dtype=torch.float32, device=x.device)
+    else:
+        q, scales = out
+        if (tuple(q.shape) != (rows, k) or tuple(scales.shape) != (rows, groups)
+                or q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32
+                or any(t.device != x.device or not t.is_contiguous() for t in out)):
+            raise ValueError("out does not match: pass the (q, scales) an earlier call returned")
+    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_FP8, q.data_ptr(), scales=scales.data_ptr(),
+             group=group or 0)
+    return (q, scales), h
+
+
+def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+                   eps: float = 1e-6, out=None, residual_out: torch.Tensor | None = None):
+    """((packed, sf, sf_perm), h): y quantised as ``quantize.quantize`` would
+    quantise it, bit for bit, and in the same three tensors (K % 64 == 0);
+    a NaN gives its 16 columns a NaN scale.  ``out``: the three tensors of an earlier
+    call of the same sizes, reused."""
+    x, weight, residual, h = _check(x, weight, residual, residual_out)
+    rows, k = x.shape
+    if k % 64:
+        raise ValueError(f"K={k} must be a multiple of 64")
+    rb, ka = -(-rows // 128), k // 64
+    if out is not None:
+        packed = out[0].view(torch.uint8).permute(2, 0, 1)
+        sf = out[1].view(torch.uint8).permute(2, 0, 1)
+        sf_perm = out[2].view(torch.uint8).permute(5, 2, 4, 0, 1, 3)
+        if (tuple(packed.shape) != (1, rows, k // 2) or tuple(sf.shape) != (1, rows, k // 16)
+                or tuple(sf_perm.shape) != (1, rb, ka, 32, 4, 4)
+                or any(t.device != x.device or not t.is_contiguous() for t in (packed, sf, sf_perm))):
+            raise ValueError("out does not match: pass the three tensors an earlier call returned")
+    else:
+        packed = torch.empty((1, rows, k // 2), dtype=torch.uint8, device=x.device)
+        sf = torch.empty((1, rows, k // 16), dtype=torch.uint8, device=x.device)
+        sf_perm = torch.empty((1, rb, ka, 32, 4, 4), dtype=torch.uint8, device=x.device)
+    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_NVFP4, packed.data_ptr(), sf_perm=sf_perm.data_ptr(),
+             sf=sf.data_ptr())
+    return (packed.permute(1, 2, 0).view(torch.float4_e2m1fn_x2),
+            sf.permute(1, 2, 0).view(torch.float8_e4m3fn),
+            sf_perm.permute(3, 4, 1, 5, 2, 0).view(torch.float8_e4m3fn)), h

@@ -18,7 +18,8 @@
  *   SF permuted scale tensor [32, 4, ceil(MN/128), 4, K/64, L] float8_e4m3fn,
  *      i.e. contiguous 512-byte atoms [L][ceil(MN/128)][K/64][32][4][4]
  *   C  [M, N, L]    float16, row-major; batch l starts at l*M*N elements
- * Requirements: K % 256 == 0, N % 8 == 0, M >= 1, all pointers 16-byte aligned.
+ * Requirements: K % 256 == 0, N % 8 == 0, M >= 1, all pointers 16-byte aligned
+ * (the products of a few tokens, nvfp4_gemv and nvfp4_moe_gemv: K % 64 == 0, any N).
  */
 #ifndef NVFP4_B200_H
 #define NVFP4_B200_H
@@ -146,6 +147,72 @@ int nvfp4_moe_grouped_gemm(const void* a_packed, int a_rows, const void* sfa_ato
  * counterpart. */
 int nvfp4_moe_combine(const void* c, int c_rows, const int* dst, const float* weights, int tokens,
                       int topk, int n, float* out, void* stream);
+
+/* Element types of x, residual, weight and out below. */
+#define NVFP4_F32 0
+#define NVFP4_F16 1
+#define NVFP4_BF16 2
+
+/* A few tokens times NVFP4 weights: out[l] = x[l] . B1[l]ᵀ, or with b2 / sf2
+ * not NULL silu(x[l] . B1[l]ᵀ) * (x[l] . B2[l]ᵀ), for l batch entries.  x [m][k]
+ * (rows ldx elements apart, batch entries x_batch) is not quantised; it enters the sums
+ * with an error of at most 2^-23 of the largest of its 16 consecutive
+ * elements, the sums are fp32, out [m][n] (rows ldo >= n elements apart, batch entries
+ * out_batch) is rounded once.  x_dtype and out_dtype are NVFP4_F32, _F16 or _BF16.
+ * Weights and permuted scale atoms as for the GEMMs, K % 64 == 0, any N.
+ * An infinity or NaN in x makes that row of out NaN.  m <= 4096; meant for
+ * m <= 16, every 16 further rows read the weights again.  `workspace`
+ * (nvfp4_gemv_workspace_bytes(), 256-byte aligned) is scratch owned by the call
+ * until it completes on `stream`.  No reference counterpart: the reference's GEMMs
+ * (nvfp4_dual_gemm/reference.py:27-77) take quantised activations. */
+int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x_batch, const void* b1,
+               const void* sf1, const void* b2, const void* sf2, void* out, int out_dtype,
+               long long ldo, long long out_batch, int m, int n, int k, int l, void* workspace,
+               size_t workspace_bytes, void* stream);
+size_t nvfp4_gemv_workspace_bytes(int m, int k, int l);
+
+/* The same with each row's own expert: out row r = t*topk + j is x_row . B_eᵀ (or
+ * gated, table2 not NULL) with e = expert_ids[r] and x_row = x row t, or x row r when
+ * x_per_pair is not 0.  Rows whose id is outside [0, num_experts) are zero.  Each
+ * expert's weights are read once for every 16 of its rows.  tokens*topk <= 256,
+ * num_experts <= 1024.  table1 / table2: device copies (64-byte aligned) of the
+ * nvfp4_moe_table_bytes() bytes that nvfp4_moe_table() writes to host memory for
+ * the experts' weights b[e] [N][K/2] and permuted scales sfb_perm[e]; they hold
+ * as long as those addresses do.  Counterpart in the reference: the grouped
+ * GEMM (nvfp4_group_gemm/reference.py:39-74), which takes quantised rows
+ * already sorted by expert. */
+int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_per_pair,
+                   const int* expert_ids, int tokens, int topk, const void* table1,
+                   const void* table2, int num_experts, void* out, int out_dtype, long long ldo,
+                   int n, int k, void* workspace, size_t workspace_bytes, void* stream);
+size_t nvfp4_moe_gemv_workspace_bytes(int tokens, int topk, int k);
+int nvfp4_moe_table(const void* const* b, const void* const* sfb_perm, int num_experts, int n,
+                    int k, void* table);
+size_t nvfp4_moe_table_bytes(int num_experts);
+
+/* What nvfp4_rms_norm writes y as. */
+#define NVFP4_NORM_PLAIN 0  /* y_dtype, rows ldy elements apart */
+#define NVFP4_NORM_FP8 1    /* e4m3 [rows][k] and fp32 scales */
+#define NVFP4_NORM_NVFP4 2  /* packed e2m1 [rows][k/2] and e4m3 scales, as nvfp4_quantize */
+
+/* h = x + residual (rounded to the residual's type; h = x when residual is NULL),
+ * y = h / sqrt(mean(h^2) + eps) * weight over the K columns of each row, in one
+ * pass.  h may be the residual itself.  The sum of squares and the root are fp64, h *
+ * r and the product with the weight are rounded to fp32 one after the other.
+ *   PLAIN  y in y_dtype
+ *   FP8    scale = amax/448 over `group` columns (32, 64 or 128, dividing K; 0: the
+ *          row), y = e4m3_rne(y/scale), scales [rows][K/group]; zeros under a
+ *          zero scale, a NaN scale for a group that holds a NaN
+ *   NVFP4  y quantised as nvfp4_quantize does (K % 64 == 0): packed in y, atoms
+ *          in sf_perm (padding rows zero), plain scales in sf_plain unless NULL;
+ *          a NaN scale for 16 columns that hold a NaN
+ * Row strides ldx, ldr, ldh, ldy in elements; K <= 32768.  Arguments of other
+ * formats are ignored.  No reference counterpart: its operands come quantised
+ * (nvfp4_dual_gemm/reference.py:113-187). */
+int nvfp4_rms_norm(const void* x, int x_dtype, long long ldx, const void* residual, int r_dtype,
+                   long long ldr, void* h, long long ldh, const void* weight, int w_dtype,
+                   double eps, int rows, int k, int format, void* y, int y_dtype, long long ldy,
+                   float* scales, int group, void* sf_perm, void* sf_plain, void* stream);
 
 /* Synchronises `stream`, then reads and clears this device's status word.
  * Returns NVFP4_ERR_TIMEOUT if a kernel gave up on a wait (bits in *bits_out,
