@@ -1226,15 +1226,17 @@ GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
 
 // CTAs of a cluster that share a tile's K: the count (a power of two, so that
 // the 128 rows divide) with the fewest K blocks on the busiest CTA, when
-// `tiles` tiles go to one CTA per SM; the smaller count unless the larger saves
-// a tenth.
+// `tiles` tiles go to one CTA per SM.  The exchange of a tile's sums counts as three
+// K blocks (about 1 us).  Measured, us with 1 / 2 / 4 / 8 CTAs, one token: 512 x 1024 4.7 /
+// 5.0 / 5.0 / 5.0, 2048 x 7168 14.7 / 10.8 / 7.9 / 6.8, 4096 x 14336 26.2 / 17.6 / 12.8 /
+// 11.9, 16384 x 7168 17.0 / 17.7 / 18.0 / 25.7; 16 tokens 7168 x 16384 28.6 / 24.2 / 31.0 / 51.4.
 int gemv_splits(long long tiles, int k_blocks, int num_sms) {
   int best = 1;
-  double least = 0;
+  long long least = 0;
   for (int s = 1; s <= kGemvMaxSplits && s <= k_blocks; s *= 2) {
     const long long clusters = num_sms / s;
-    const double load = (double)((tiles + clusters - 1) / clusters) * ((k_blocks + s - 1) / s);
-    if (s == 1 || load < 0.9 * least) best = s, least = load;
+    const long long load = (tiles + clusters - 1) / clusters * ((k_blocks + s - 1) / s + (s > 1 ? 3 : 0));
+    if (s == 1 || load < least) best = s, least = load;
   }
   return best;
 }
@@ -1268,19 +1270,21 @@ int launch_chained(Kern kern, dim3 grid, int threads, int smem, int cluster, cud
   return check_launch(what);
 }
 
-template <bool kDual, bool kMoe, int kTmemCols>
+template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
 int launch_gemv(DeviceState* d, int slot, const GemvParams& p, int smem, long long tiles, cudaStream_t stream) {
-  auto kern = gemv_kernel<kDual, kMoe, kTmemCols>;
-  int rc = set_smem_once(d, slot, kern, kGemvSmem);
+  auto kern = gemv_kernel<kDual, kMoe, kSelf, kTmemCols>;
+  int rc = set_smem_once(d, slot, kern, 220 * 1024);
   if (rc) return rc;
-  const int chunks = ((p.k_blocks + p.splits - 1) / p.splits + kExpandBlocks - 1) / kExpandBlocks;
-  const int rows = kMoe ? p.pairs : p.l * p.m;
-  rc = launch_chained(gemv_expand_kernel<kMoe>, dim3((unsigned)rows, (unsigned)(chunks * p.splits), 1), kExpandThreads, 0,
-                      1, stream, p, "gemv_expand_kernel");
-  if (rc) return rc;
+  if constexpr (!kSelf) {
+    const int chunks = ((p.k_blocks + p.splits - 1) / p.splits + kExpandBlocks - 1) / kExpandBlocks;
+    const int rows = kMoe ? p.pairs : p.l * p.m;
+    rc = launch_chained(gemv_expand_kernel<kMoe>, dim3((unsigned)rows, (unsigned)(chunks * p.splits), 1), kExpandThreads, 0,
+                        1, stream, p, "gemv_expand_kernel");
+    if (rc) return rc;
+  }
   const long long most = d->num_sms / p.splits;
   const long long clusters = tiles < most ? tiles : most;
-  return launch_chained(kern, dim3((unsigned)(clusters * p.splits), 1, 1), kGemvThreads, smem, p.splits, stream, p,
+  return launch_chained(kern, dim3((unsigned)(clusters * p.splits), 1, 1), gemv_threads(kSelf), smem, p.splits, stream, p,
                         "gemv_kernel");
 }
 
@@ -1292,10 +1296,18 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.row_blocks = (p.n + kBM - 1) / kBM;
   p.passes = (p.m + kGemvTokens - 1) / kGemvTokens;
   const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
-  p.group_rows = rows < kGemvTokens ? rows : kGemvTokens;
   const long long tiles = (long long)groups * p.row_blocks;
   p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms);
+  if (getenv("GEMV_S")) p.splits = atoi(getenv("GEMV_S"));
   while (p.splits > p.k_blocks) p.splits /= 2;
+  const int span = (p.k_blocks + p.splits - 1) / p.splits;
+  bool self = kMoe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens && p.m * span <= 16;
+  if (getenv("GEMV_SELF")) self = (kMoe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens) && atoi(getenv("GEMV_SELF"));
+  p.room = self ? (kMoe ? 2 : kGemvSelfTokens) : kGemvTokens;
+  // experts: twice the average of an expert's rows, so that the x slots are not sized for what hardly ever comes
+  if (kMoe && !self)
+    while (p.room > 4 && (long long)p.room * p.experts >= 4LL * p.pairs) p.room /= 2;
+  p.group_rows = rows < p.room ? rows : p.room;
   const GemvSpace sp = gemv_space(kMoe, kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   p.groups = reinterpret_cast<GemvGroups*>(ws);
@@ -1305,15 +1317,26 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.wait_limit = wait_limit_cycles();
   constexpr int kMats = kDual ? 2 : 1;
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
+  const int n_pad = (p.group_rows * kGemvTerms + 15) / 16 * 16;
   const int sums = p.splits > 1 ? kMats * p.group_rows * kBM * (int)sizeof(float) : 0;
-  p.x_slots = x_bytes > 8192 ? 2 : kGemvMaxXSlots;
-  p.w_slots = (kGemvSmem - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
+  int budget = p.group_rows > 8 ? 216 * 1024 : kGemvSmem;
+  if (getenv("GEMV_B")) budget = atoi(getenv("GEMV_B")) * 1024;
+  p.x_slots = self ? (p.group_rows <= 2 ? 8 : 4) : 4;
+  if (getenv("GEMV_X") && !self) p.x_slots = atoi(getenv("GEMV_X"));
+  p.w_slots = (budget - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
   if (p.w_slots > kGemvMaxWSlots) p.w_slots = kGemvMaxWSlots;
+  p.w_slots &= ~1;
   const int smem = 1024 + p.w_slots * kGemvWBytes + p.x_slots * x_bytes + sums;
-  const int cols = kMats * ((p.group_rows * kGemvTerms + 15) / 16 * 16) + 16 * (p.w_slots + p.x_slots);
-  const int base = 32 + (kDual ? 4 : 0) + (kMoe ? 2 : 0);
-  if (cols <= 256) return launch_gemv<kDual, kMoe, 256>(d, base, p, smem, tiles, stream);
-  return launch_gemv<kDual, kMoe, 512>(d, base + 1, p, smem, tiles, stream);
+  // TMEM: two accumulators (twice where there is room) and the slots' scales
+  const int sf_cols = kGemvSfCols * p.w_slots;
+  p.acc_bufs = 4 * n_pad + sf_cols <= 256 ? 2 : 2 * n_pad + sf_cols <= 256 ? 1 : 4 * n_pad + sf_cols <= 512 ? 2 : 1;
+  const int cols = p.acc_bufs * 2 * n_pad + sf_cols;
+  if (p.w_slots < 2 || cols > (self ? 256 : 512))
+    return fail(NVFP4_ERR_SHAPE, "%d weight slots, %d TMEM columns", p.w_slots, cols);
+  const int base = 32 + (kDual ? 6 : 0) + (kMoe ? 3 : 0);
+  if (self) return launch_gemv<kDual, kMoe, true, 256>(d, base, p, smem, tiles, stream);
+  if (cols <= 256) return launch_gemv<kDual, kMoe, false, 256>(d, base + 1, p, smem, tiles, stream);
+  return launch_gemv<kDual, kMoe, false, 512>(d, base + 2, p, smem, tiles, stream);
 }
 
 int dtype_size(int t) { return t == kDtF32 ? 4 : 2; }

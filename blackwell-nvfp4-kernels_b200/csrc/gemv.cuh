@@ -4,17 +4,16 @@
 // nothing that an fp32 sum keeps; sums are fp32.
 //
 // Mathematics.  The block-scaled MMA (tcgen05.mma kind::mxf4nvf4) multiplies
-// e2m1 by e2m1, so x is written as a sum of kGemvTerms = 8 e2m1 digits in base 8.  For
-// 16 consecutive elements with largest magnitude a, let s be the smallest
-// power of two with a <= 4.5 s.  Then
-//   t_1 = x / s,   q_j = e2m1(t_j) (nearest),   t_(j+1) = 8 (t_j - q_j),
-//   x = s (q_1 + q_2 / 8 + ... + q_8 / 8^7) + error,   |error| <= s / 2 / 8^7 < 2^-23 a.
-// It converges because below 5 the e2m1 values are at most 1 apart: |t_j| <= 4.5
-// gives |t_j - q_j| <= 1/2 and |t_(j+1)| <= 4.  Every step is exact in fp32, s
-// is an e4m3 scale (of all eight digits, 2^-6 <= s <= 2^8 after x is multiplied by a power
-// of two 2^e chosen for the token and K range), and the MMA's products are exact.  The digits
-// are eight rows of the MMA's B operand, the weights are its A operand (128
-// rows), read by the tensor core as they are stored:
+// e2m1 by e2m1, so x is written as eight balanced base-8 digits.  For 16
+// consecutive elements with largest magnitude a, let s be the smallest power of two
+// with a <= 1.5 s.  Then
+//   x = s (q_1 + q_2 / 8 + ... + q_8 / 8^7) + error,   q_j in {-2, -1.5, ..., 1.5},
+// where the q_j are the digits (in halves) of the integer nearest to 2 * 8^7 x / s:
+// they are e2m1 values, and |error| <= s / 4 / 8^7 = 2^-23 s < 2^-22 a.  s is an
+// e4m3 scale (of all eight digits; 2^-6 <= s <= 2^8 after x is multiplied by a
+// power of two 2^e chosen for the token and K range), and the MMA's products are exact.
+// The digits are eight rows of the MMA's B operand, the weights are its A
+// operand (128 rows), read by the tensor core as they are stored:
 //   D[row][8 token + j] = sum over k of W[row][k] s q_(j+1),
 //   y[token][row] = 2^-e (D_0 + (D_1 + (D_2 + ...) / 8) / 8).
 // Nothing touches the weights between HBM and the tensor core, so a token
@@ -26,9 +25,11 @@
 // An infinite or NaN element makes its 16 elements' scale NaN, and with it
 // every output of that token.
 //
-// Two kernels.  gemv_expand_kernel writes the digits and scales as images of the
-// shared memory that the MMAs read.  gemv_kernel streams the weights.  It may
-// start loading them before the expansion is done: the expansion lets
+// With few tokens gemv_kernel expands x itself, four warps of each CTA for its
+// part of K, while the first weights are on their way.  With more that would
+// be the slowest part (about 300 warp instructions for a token's 256
+// elements), and gemv_expand_kernel does it once, as images of the shared memory that the MMAs
+// read; gemv_kernel may then load weights before the expansion is done, because the expansion lets
 // it start only after its own wait for all earlier work in the stream.
 #pragma once
 #include <cuda.h>
@@ -57,7 +58,7 @@ struct alignas(64) GemvExpert {
   const uint8_t* sf;
 };
 
-// Groups of an expert call, written by the expansion: an expert and up to 16 of its rows.
+// Groups of an expert call: an expert and up to 16 of its rows.
 struct GemvGroups {
   int count;
   int expert[kGemvMaxPairs];
@@ -79,8 +80,8 @@ struct GemvParams {
   int k_blocks, row_blocks;              // 256-deep K blocks, 128-row blocks
   int passes;                            // groups of 16 tokens of a batch entry
   int splits;                            // CTAs of a cluster, each with a part of K
-  int group_rows;                        // tokens of the largest group
-  int w_slots, x_slots;                  // shared-memory ring slots
+  int room, group_rows;                  // tokens that a group can have, and the largest has
+  int w_slots, x_slots, acc_bufs;        // shared-memory ring slots, accumulators
   // expansion
   float* back;                           // [group][16][splits]: 2^-e
   uint8_t* image;                        // [k_block][group]: digits, scale atoms
@@ -117,50 +118,163 @@ __device__ __forceinline__ size_t gemv_image_at(int kb, int rows_all, int groups
 // ---------------------------------------------------------------------------
 // Expansion
 // ---------------------------------------------------------------------------
-constexpr int kExpandThreads = 128;                       // a thread has 16 elements
-constexpr int kExpandBlocks = kExpandThreads / 16;        // K blocks of a CTA
+constexpr int kExpandThreads = 256;                       // a warp has a K block, a thread 8 elements
+constexpr int kExpandBlocks = kExpandThreads / 32;        // K blocks of a CTA
 
-// Eight consecutive elements as fp32.
-__device__ __forceinline__ void gemv_load8(const GemvParams& p, int64_t at, float (&f)[8]) {
-  uint32_t v[8];
-  if (p.x_dtype == kDtF32) {
-    const uint32_t* q = static_cast<const uint32_t*>(p.x) + at;
-    if (p.x_vec) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(q)), b = __ldg(reinterpret_cast<const uint4*>(q) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// Eight consecutive elements as they lie in memory (b: fp32 only).  kVec: 16-byte aligned.
+struct Raw8 { uint4 a, b; };
+template <bool kWide, bool kVec>
+__device__ __forceinline__ Raw8 gemv_raw8(const void* x, int64_t at) {
+  Raw8 r;
+  r.b = make_uint4(0, 0, 0, 0);
+  if constexpr (kWide) {
+    const uint32_t* q = static_cast<const uint32_t*>(x) + at;
+    if constexpr (kVec) {
+      r.a = __ldg(reinterpret_cast<const uint4*>(q)), r.b = __ldg(reinterpret_cast<const uint4*>(q) + 1);
     } else {
-      #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __ldg(q + i);
+      r.a = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+      r.b = make_uint4(__ldg(q + 4), __ldg(q + 5), __ldg(q + 6), __ldg(q + 7));
     }
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i]);
-    return;
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(x) + at;
+    if constexpr (kVec) {
+      r.a = __ldg(reinterpret_cast<const uint4*>(q));
+    } else {
+      uint32_t v[4];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
+      r.a = make_uint4(v[0], v[1], v[2], v[3]);
+    }
   }
-  const uint16_t* q = static_cast<const uint16_t*>(p.x) + at;
-  if (p.x_vec) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(q));
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  return r;
+}
+
+// As fp32.
+__device__ __forceinline__ void widen8(const Raw8& r, int dtype, float (&f)[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if (dtype == kDtF32) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+  } else if (dtype == kDtBF16) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   } else {
     #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
-  }
-  #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (p.x_dtype == kDtBF16) {
-      f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-    } else {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       f[2 * i] = t.x, f[2 * i + 1] = t.y;
     }
   }
 }
 
-__device__ __forceinline__ void take_largest(uint32_t& top, float f) {   // of the finite magnitudes, as bits
-  const uint32_t bits = __float_as_uint(f) & 0x7fffffffu;
-  if (bits < 0x7f800000u && bits > top) top = bits;
+// Calls f with the loader of x's type and alignment: the choice is made once, outside
+// of the loops, so that their loads can be in flight together.
+template <class F>
+__device__ __forceinline__ void gemv_with_loader(const GemvParams& p, F f) {
+  const void* x = p.x;
+  if (p.x_dtype == kDtF32) {
+    if (p.x_vec) f([x](int64_t at) { return gemv_raw8<true, true>(x, at); });
+    else f([x](int64_t at) { return gemv_raw8<true, false>(x, at); });
+  } else {
+    if (p.x_vec) f([x](int64_t at) { return gemv_raw8<false, true>(x, at); });
+    else f([x](int64_t at) { return gemv_raw8<false, false>(x, at); });
+  }
 }
 
-// Pairs of one expert in ascending order, 16 at a time; one warp, the result in shared memory.
+// Largest finite magnitude (bits) of eight elements.
+__device__ __forceinline__ uint32_t largest8(const Raw8& r, int dtype) {
+  float f[8];
+  widen8(r, dtype, f);
+  uint32_t top = 0;
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = __float_as_uint(f[i]) & 0x7fffffffu;
+    top = max(top, bits < 0x7f800000u ? bits : 0u);
+  }
+  return top;
+}
+
+// The exponent that takes a largest magnitude (bits) into [2^7, 2^8): scales
+// reach 2^8 at most; as far as it and its inverse are normal numbers.
+__device__ __forceinline__ int gemv_exponent(uint32_t top) { return min(7 - ((int)(top >> 23) - 127), 126); }
+
+// Transposes 8 words of 8 nibbles: word c's nibble r becomes word r's nibble c.
+__device__ __forceinline__ void transpose_nibbles(uint32_t* w) {
+  #pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t a = w[r], b = w[r + 4];
+    w[r] = __byte_perm(a, b, 0x5410), w[r + 4] = __byte_perm(a, b, 0x7632);
+  }
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i < 2 ? i : i + 2;
+    const uint32_t a = w[r], b = w[r + 2];
+    w[r] = __byte_perm(a, b, 0x6240), w[r + 2] = __byte_perm(a, b, 0x7351);
+  }
+  #pragma unroll
+  for (int r = 0; r < 8; r += 2) {
+    const uint32_t a = w[r], b = w[r + 1];
+    w[r] = (a & 0x0f0f0f0fu) | ((b & 0x0f0f0f0fu) << 4);
+    w[r + 1] = ((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
+  }
+}
+
+// Digits of a warp's 256 elements, eight in each lane (two lanes a block of
+// 16): store(j, eight codes) for j = 0..7; returns the four scale bytes of 64 elements,
+// valid in lanes 0, 8, 16 and 24.  `up`: 2^e.
+template <class Store>
+__device__ __forceinline__ uint32_t gemv_digits(float (&v)[8], float up, Store store) {
+  uint32_t amax = 0;
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] *= up;
+    amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  const bool finite = amax < 0x7f800000u;
+  // s = 2^q: the smallest with amax <= 1.5 s, in [2^-6, 2^8]
+  const int q = max((int)(amax >> 23) - 127 + ((amax & 0x7fffffu) > 0x400000u ? 1 : 0), -6);
+  const float units = finite ? exp2_int(22 - q) : 0.f;    // of s / 2 / 8^7
+  uint32_t w[8];
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // balanced base-8 digits: 4 added to each makes them the 3-bit fields of one number
+    const uint32_t y = (uint32_t)(__float2int_rn(finite ? v[i] * units : 0.f) + 0x924924);
+    uint32_t x = (y & 0xfffu) | ((y & 0xfff000u) << 4);
+    x = (x & 0x003f003fu) | ((x & 0x0fc00fc0u) << 2);
+    x = (x & 0x07070707u) | ((x & 0x38383838u) << 1);     // fields f in nibbles
+    // code of (f - 4) / 2: f - 4 for f >= 4, else sign and 4 - f
+    const uint32_t neg = (~x >> 2) & 0x11111111u;
+    w[i] = (((x & 0x33333333u) ^ (neg * 3u)) + neg) | (neg << 3);
+  }
+  transpose_nibbles(w);
+  #pragma unroll
+  for (int j = 0; j < kGemvTerms; ++j) store(j, w[7 - j]);
+  const uint32_t s8 = finite ? (uint32_t)(q + 7) << 3 : 0x7fu;   // e4m3 of 2^q, or NaN
+  const uint32_t pair = s8 | (__shfl_down_sync(0xffffffffu, s8, 2) << 8);
+  return pair | (__shfl_down_sync(0xffffffffu, pair, 4) << 16);
+}
+
+// Offset of lane's four bytes of digit j among a token's 8 x 128 bytes: 16-byte
+// pieces exchanged as the 128-byte swizzle has them.
+__device__ __forceinline__ int gemv_digit_at(int lane, int j) { return j * 128 + (((lane >> 2) ^ j) << 4) + (lane & 3) * 4; }
+
+// Where digit row `row` of a group has its scale word in an atom.
+__device__ __forceinline__ int gemv_scale_at(int row) { return (row % 32) * 16 + (row / 32) * 4; }
+
+// Digits and scales of one token's 256 elements (a warp's) to an image: `token`
+// its digits, `atoms` the group's scale atoms.  Lane 8a + j writes digit j's scales of atom a.
+__device__ __forceinline__ void gemv_put(float (&v)[8], float up, uint8_t* token, uint8_t* atoms, int place) {
+  const int lane = (int)(threadIdx.x & 31u);
+  const uint32_t four = gemv_digits(v, up, [&](int j, uint32_t w) {
+    *reinterpret_cast<uint32_t*>(token + gemv_digit_at(lane, j)) = w;
+  });
+  const uint32_t mine = __shfl_sync(0xffffffffu, four, lane & 24);
+  *reinterpret_cast<uint32_t*>(atoms + (lane >> 3) * kSfAtom + gemv_scale_at(place * kGemvTerms + (lane & 7))) = mine;
+}
+
+// Pairs of one expert in ascending order, p.room at a time; one warp, the result in shared memory.
 __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups& out, int* seen, int* open,
                                                  int* group_of, int* place_of) {
   const int lane = (int)(threadIdx.x & 31u);
@@ -175,7 +289,7 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
     const uint32_t same = __match_any_sync(0xffffffffu, valid ? id : -1);
     const int before = valid ? seen[id] : 0, at = before + __popc(same & lt);
     const int old = valid && before > 0 ? open[id] : 0;
-    const bool first = valid && at % kGemvTokens == 0;
+    const bool first = valid && at % p.room == 0;
     const uint32_t firsts = __ballot_sync(0xffffffffu, first);
     int grp = groups + __popc(firsts & lt);
     const uint32_t mine = firsts & same & (lt | (1u << lane));   // the group's first row, if it is among these 32
@@ -185,7 +299,7 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
     __syncwarp();
     if (valid) atomicAdd(&out.rows[grp], 1);
     if (valid && (same >> lane) == 1u) seen[id] = at + 1, open[id] = grp;   // the expert's last row among these
-    if (i < p.pairs) group_of[i] = valid ? grp : -1, place_of[i] = at % kGemvTokens;
+    if (i < p.pairs) group_of[i] = valid ? grp : -1, place_of[i] = at % p.room;
     groups += __popc(firsts);
     __syncwarp();
   }
@@ -209,7 +323,7 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
 
 // grid: (row of x, chunk of 8 K blocks of a split).  A CTA takes the largest magnitude
 // of its row in the whole split (every CTA of the split reads it: a few KB from L2),
-// then each thread expands 16 elements.
+// then each warp expands one K block.
 template <bool kMoe>
 __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __grid_constant__ GemvParams p) {
   __shared__ uint32_t s_top[kExpandThreads / 32];
@@ -255,103 +369,95 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
   const int kb0 = p.k_blocks * split / p.splits, kb1 = p.k_blocks * (split + 1) / p.splits;
   if (kb0 + chunk * kExpandBlocks >= kb1) return;
 
-  // this thread's 16 elements, and the largest of the split
-  const int kb = kb0 + chunk * kExpandBlocks + tid / 16, b = tid % 16;
-  const int k0 = kb * kBK + b * 16;
-  const bool mine = kb < kb1 && k0 < p.k;
-  float v[16];
+  // this thread's elements, and the largest of the split
+  const int kb = kb0 + chunk * kExpandBlocks + warp, k0 = kb * kBK + lane * 8;
+  Raw8 raw;
+  raw.a = raw.b = make_uint4(0, 0, 0, 0);
   uint32_t top = 0;
-  {
-    float lo[8], hi[8];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
-    if (mine) gemv_load8(p, src + k0, lo), gemv_load8(p, src + k0 + 8, hi);
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = lo[i], v[8 + i] = hi[i];
-  }
-  for (int c = kb0 * (kBK / 8) + tid; c < min(kb1 * kBK, p.k) / 8; c += kExpandThreads) {
-    float f[8];
-    gemv_load8(p, src + (int64_t)c * 8, f);
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) take_largest(top, f[i]);
-  }
+  gemv_with_loader(p, [&](auto load) {
+    if (kb < kb1 && k0 < p.k) raw = load(src + k0);
+    const int c1 = min(kb1 * kBK, p.k) / 8;
+    for (int c = kb0 * (kBK / 8) + tid; c < c1; c += 4 * kExpandThreads) {
+      Raw8 r[4];
+      #pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = load(src + (int64_t)(c + u * kExpandThreads < c1 ? c + u * kExpandThreads : c) * 8);
+      #pragma unroll
+      for (int u = 0; u < 4; ++u) top = max(top, largest8(r[u], p.x_dtype));
+    }
+  });
+  float v[8];
+  widen8(raw, p.x_dtype, v);
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
   #pragma unroll
   for (int i = 0; i < kExpandThreads / 32; ++i) top = max(top, s_top[i]);
-  // the largest magnitude goes into [2^9, 2^10): scales reach 2^8 at most
-  const int e = min(9 - ((int)(top >> 23) - 127), 126);
+  const int e = gemv_exponent(top);
   if (chunk == 0 && tid == 0) p.back[((int64_t)group * kGemvTokens + place) * p.splits + split] = exp2_int(-e);
-
-  const float up = exp2_int(e);
-  uint32_t amax = 0;
-  bool finite = true;
-  #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    finite = finite && (__float_as_uint(v[i]) & 0x7fffffffu) < 0x7f800000u;
-    v[i] *= up;
-    take_largest(amax, v[i]);
-  }
-  // s = 2^q: the smallest with amax <= 4.5 s (1.125 * 2^(q + 2)), in [2^-6, 2^8]
-  int q = (int)(amax >> 23) - 127 - ((amax & 0x7fffffu) <= 0x100000u ? 2 : 1);
-  q = max(q, -6);
-  const float down = exp2_int(-q);
-  #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = finite ? v[i] * down : 0.f;
+  if (kb >= kb1) return;
   uint8_t* const image = p.image + gemv_image_at(kb, rows_all, groups_all, before, group);
-  uint8_t* const digits = image + place * kGemvTokenBytes + (b & 1) * 8;
-  #pragma unroll
-  for (int j = 0; j < kGemvTerms; ++j) {
-    uint32_t word[2] = {0u, 0u};
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t two = e2m1x2(v[2 * i], v[2 * i + 1]);
-      word[i / 4] |= two << (8 * (i % 4));
-      uint32_t h;
-      asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(two));
-      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      v[2 * i] = (v[2 * i] - d.x) * 8.f;
-      v[2 * i + 1] = (v[2 * i + 1] - d.y) * 8.f;
-    }
-    // row j of the token's 8 x 128 bytes, 16-byte pieces exchanged as the 128-byte swizzle has them
-    if (mine) *reinterpret_cast<uint2*>(digits + j * 128 + (((b >> 1) ^ j) << 4)) = make_uint2(word[0], word[1]);
-  }
-  const uint32_t s8 = finite ? (uint32_t)(q + 7) << 3 : 0x7fu;   // e4m3 of 2^q, or NaN
-  const uint32_t pair = s8 | (__shfl_down_sync(0xffffffffu, s8, 1) << 8);
-  const uint32_t four = pair | (__shfl_down_sync(0xffffffffu, pair, 2) << 16);
-  if (mine && b % 4 == 0) {
-    uint8_t* const atom = image + rows * kGemvTokenBytes + (b / 4) * kSfAtom;
-    #pragma unroll
-    for (int j = 0; j < kGemvTerms; ++j) {
-      const int row = place * kGemvTerms + j;
-      *reinterpret_cast<uint32_t*>(atom + (row % 32) * 16 + (row / 32) * 4) = four;
-    }
-  }
+  gemv_put(v, exp2_int(e), image + place * kGemvTokenBytes, image + rows * kGemvTokenBytes, place);
 }
 
 // ---------------------------------------------------------------------------
 // Products
 // ---------------------------------------------------------------------------
 constexpr int kGemvWBytes = kBM * kBK / 2 + kSfStageBytes;   // a weight slot: 128 rows x 256, scale atoms
-constexpr int kGemvMaxWSlots = 8, kGemvMaxXSlots = 4;
-constexpr int kGemvThreads = 7 * 32;     // epilogue warps 0-3, weights 4, x 5, MMA and TMEM 6
+constexpr int kGemvSfCols = 32;          // TMEM columns of a weight slot: its scales and x's
+constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // x slots a power of two
+constexpr int kGemvSelfTokens = 4;       // largest group that gemv_kernel expands itself
+// tiles that the expansion may be ahead of the epilogue: two accumulators, x slots of one K block each
+constexpr int kGemvAhead = kGemvMaxXSlots + 4;
+constexpr int kGemvSelfPairs = 32;       // and the most rows of an expert call
+// warps: epilogue 0-3, expansion 4-11 (without it x copies: 4), then weights, two for the MMAs
+constexpr int gemv_threads(bool self) { return 32 * (self ? 15 : 8); }
 
 // Copy one scale atom into TMEM: row i to lane i of each lane quadrant, 4 columns.
 __device__ __forceinline__ void tc_cp_32x128b_x4(uint32_t taddr, uint64_t s_desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
 }
 
+// Hints: bring a weight slot's bytes into L2.
+__device__ __forceinline__ void prefetch_l2_3d(const void* tmap, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tmap), "r"(c0), "r"(c1),
+               "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// Store to shared memory of any CTA of the cluster, its bytes counted on an
+// mbarrier there: the data and the signal in one, no fence.
+__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr),
+               "r"(__float_as_uint(v)), "r"(cluster_bar)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // What a cluster works on: tile t of the call.
 struct GemvTile { int group, row_block, batch, rows, before, expert; };
 
-template <bool kMoe>
-__device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, int t) {
+// Groups of a small expert call, made by each CTA for itself.
+struct GemvSmallGroups {
+  int count;
+  int expert[kGemvSelfPairs], rows[kGemvSelfPairs];
+  int pair[kGemvSelfPairs][kGemvSelfTokens];
+};
+
+template <bool kMoe, bool kSelf>
+__device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSmallGroups& small, int t) {
   GemvTile r;
   if constexpr (kMoe) {
     r.group = t / p.row_blocks, r.row_block = t % p.row_blocks, r.batch = 0;
-    r.expert = __ldcg(&p.groups->expert[r.group]);
-    r.rows = __ldcg(&p.groups->rows[r.group]), r.before = __ldcg(&p.groups->before[r.group]);
+    if constexpr (kSelf) {
+      r.expert = small.expert[r.group], r.rows = small.rows[r.group], r.before = 0;
+    } else {
+      r.expert = __ldcg(&p.groups->expert[r.group]);
+      r.rows = __ldcg(&p.groups->rows[r.group]), r.before = __ldcg(&p.groups->before[r.group]);
+    }
   } else {
     // groups of the same weights next to one another: they share them in L2
     const int pass = t % p.passes, rest = t / p.passes;
@@ -366,22 +472,26 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, int t) {
 // A cluster of `splits` CTAs owns a 128-row block and a group; each CTA has a
 // part of K.  Shared memory holds a ring of weight slots (one matrix' K block,
 // 18 KB) and a ring of x slots; it is kept to half of the SM's, so that the next
-// kernel's CTAs can be resident and start their loads while this one ends.  The sums of
+// kernel's CTAs can be resident and get ready while this one ends.  The sums of
 // the CTAs of a cluster meet in distributed shared memory: each CTA owns 128 / splits rows,
 // gets the others' sums for them and adds them in the order of the CTAs.
-template <bool kDual, bool kMoe, int kTmemCols>
-__global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const __grid_constant__ GemvParams p) {
+template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
+__global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_constant__ GemvParams p) {
   constexpr int kMats = kDual ? 2 : 1;
+  constexpr int kWWarp = kSelf ? 12 : 5, kMmaWarp = kWWarp + 1;   // and kMmaWarp + 1
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_w_full[kGemvMaxWSlots], bar_w_free[kGemvMaxWSlots];
   __shared__ uint64_t bar_x_full[kGemvMaxXSlots], bar_x_free[kGemvMaxXSlots];
-  __shared__ uint64_t bar_acc_full, bar_acc_free, bar_drain;
+  __shared__ uint64_t bar_acc_full[2], bar_acc_free[2], bar_drain[2];
   __shared__ uint64_t bar_sums, bar_sums_free;            // this CTA's rows: all sums there; its sums taken everywhere
   __shared__ uint32_t s_tmem_base;
   __shared__ volatile int s_abort;
+  __shared__ uint32_t s_top[kGemvSelfTokens];             // expansion: largest magnitudes
+  __shared__ float s_back[kGemvAhead][kGemvSelfTokens];   // and 2^-e of the tokens of tile index % kGemvAhead
+  __shared__ GemvSmallGroups s_small;
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int warp = (int)threadIdx.x >> 5;
+  const int warp = (int)threadIdx.x >> 5, lane = (int)(threadIdx.x & 31u);
   const int splits = p.splits;
   const int rank = splits > 1 ? (int)cluster_ctarank() : 0;
   const int cluster = (int)blockIdx.x / splits, clusters = (int)gridDim.x / splits;
@@ -395,38 +505,79 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.w_slots; ++i) mbar_init(smem_u32(&bar_w_full[i]), 1), mbar_init(smem_u32(&bar_w_free[i]), 1);
-    for (int i = 0; i < p.x_slots; ++i) mbar_init(smem_u32(&bar_x_full[i]), 1), mbar_init(smem_u32(&bar_x_free[i]), 1);
-    mbar_init(smem_u32(&bar_acc_full), 1);
-    mbar_init(smem_u32(&bar_acc_free), 4);
-    mbar_init(smem_u32(&bar_drain), 1);
-    mbar_init(smem_u32(&bar_sums), splits);
+    for (int i = 0; i < p.x_slots; ++i) {
+      mbar_init(smem_u32(&bar_x_full[i]), kSelf ? p.group_rows : 1);
+      mbar_init(smem_u32(&bar_x_free[i]), kMats);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 2);
+      mbar_init(smem_u32(&bar_acc_free[i]), 4);
+      mbar_init(smem_u32(&bar_drain[i]), 1);
+    }
+    mbar_init(smem_u32(&bar_sums), 1);
     mbar_init(smem_u32(&bar_sums_free), splits);
     s_abort = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == 6) tmem_alloc<kTmemCols>(smem_u32(&s_tmem_base));
+  if (warp == kMmaWarp) tmem_alloc<kTmemCols>(smem_u32(&s_tmem_base));
+  if constexpr (kMoe) griddep_wait();                     // the experts' ids, or the groups from the expansion
+  if constexpr (kMoe && kSelf) {
+    // rows of one expert in ascending order, p.room at a time
+    if (warp == 0) {
+      const uint32_t lt = (1u << lane) - 1u;
+      const int id = lane < p.pairs ? __ldg(p.ids + lane) : -1;
+      const bool valid = (unsigned)id < (unsigned)p.experts;
+      const uint32_t same = __match_any_sync(0xffffffffu, valid ? id : -1);
+      const int at = __popc(same & lt);
+      const bool first = valid && at % p.room == 0;
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      const uint32_t mine = firsts & same & (lt | (1u << lane));
+      const int from = valid ? 31 - __clz(mine) : lane;
+      const int grp = __shfl_sync(0xffffffffu, __popc(firsts & lt), from);
+      if (valid) s_small.pair[grp][at % p.room] = lane;
+      if (first) s_small.expert[grp] = id, s_small.rows[grp] = min(p.room, __popc(same) - at);
+      if (lane == 0) s_small.count = __popc(firsts);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   if (splits > 1) cluster_sync();                         // the others' barriers exist
   tc_fence_after();
   const uint32_t tmem = s_tmem_base;
   const AbortCtl ctl{&s_abort, p.status, p.wait_limit};
-  // experts: the groups come from the expansion
-  if (kMoe) griddep_wait();
   if (threadIdx.x == 0) griddep_launch_dependents();
-  const int tiles = kMoe ? __ldcg(&p.groups->count) * p.row_blocks : p.l * p.passes * p.row_blocks;
+  const int tiles = !kMoe ? p.l * p.passes * p.row_blocks
+                          : (kSelf ? s_small.count : __ldcg(&p.groups->count)) * p.row_blocks;
   const int atoms_all = p.k / kKStep;                     // 64-deep atoms of a 128-row block
 
-  if (warp == 4) {
+  if (warp == kWWarp) {
     // ------------------------------------------------------------ weights
     if (elect_one()) {
       const uint64_t pol = policy_evict_normal();
       int slot = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
+      if constexpr (kSelf && !kMoe) {
+        // the first slots' bytes towards L2 while earlier kernels end (they may still write them: a
+        // prefetch is only a hint, and L2 is where everybody sees them), the loads after the wait
+        if (cluster < tiles) {
+          const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, cluster);
+          const size_t atom0 = ((size_t)tc.batch * p.row_blocks + tc.row_block) * (size_t)atoms_all;
+          for (int kb = kb0; kb < min(kb1, kb0 + p.w_slots / kMats); ++kb) {
+            const int atoms = min(kBK / kKStep, atoms_all - kb * (kBK / kKStep));
+            prefetch_l2_3d(&p.map1, kb * (kBK / 2), tc.row_block * kBM, tc.batch);
+            prefetch_l2(p.sf1 + (atom0 + (size_t)kb * (kBK / kKStep)) * kSfAtom, atoms * kSfAtom);
+            if constexpr (kDual) {
+              prefetch_l2_3d(&p.map2, kb * (kBK / 2), tc.row_block * kBM, tc.batch);
+              prefetch_l2(p.sf2 + (atom0 + (size_t)kb * (kBK / kKStep)) * kSfAtom, atoms * kSfAtom);
+            }
+          }
+        }
+        griddep_wait();
+      }
       for (int t = cluster; t < tiles && ok; t += clusters) {
-        const GemvTile tc = gemv_tile<kMoe>(p, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
         const void *map[2] = {&p.map1, &p.map2};
         const uint8_t* sf[2] = {p.sf1, p.sf2};
         if constexpr (kMoe) {
@@ -457,17 +608,97 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const __grid_constan
         for (int s = 0; s < p.w_slots; ++s)
           if ((issued >> s) & 1u) ctl.drain_copies(smem_u32(&bar_w_full[s]), (last_phase >> s) & 1u);
     }
-  } else if (warp == 5) {
-    // ------------------------------------------------------------ x
-    if (elect_one()) {
-      griddep_wait();                                     // the expansion is done
+  } else if (warp >= 4 && warp < kWWarp) {
+    griddep_wait();                                       // x, or the expansion of it
+    if constexpr (kSelf) {
+      // ---------------------------------------------------------- x: expanded here
+      // a warp takes one token's K block at a time, a lane 8 elements; 8 of them a
+      // round.  The warps end each round together: a slot's next user then cannot wait for
+      // its barrier before this round's user has (the parity of a phase says nothing
+      // about the phase two before), and all give up if one has to.
+      const int me = warp - 4, tid = (int)threadIdx.x - 128;
+      const int span = kb1 - kb0;
+      const int slot_mask = p.x_slots - 1, slot_bits = __popc(slot_mask);
+      int seen = -1, done = 0, index = 0;                 // group whose s_top is there; K blocks before this tile
+      bool ok = true;
+      for (int t = cluster; t < tiles && ok; t += clusters, done += span, ++index) {
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        auto x_at = [&](int tok) -> int64_t {
+          if constexpr (kMoe) {
+            const int pr = s_small.pair[tc.group][tok];
+            return (int64_t)(p.x_per_pair ? pr : pr / p.topk) * p.ldx;
+          }
+          return (int64_t)tc.batch * p.x_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldx;
+        };
+        const int items = span * tc.rows;
+        // an item's elements, loaded a round ahead
+        auto load_item = [&](auto load, int i) {
+          const int k0 = (kb0 + i / tc.rows) * kBK + lane * 8, tok = i % tc.rows;
+          Raw8 r;
+          r.a = r.b = make_uint4(0, 0, 0, 0);
+          if (i < items && k0 < p.k) r = load(x_at(tok) + k0);
+          return r;
+        };
+        Raw8 next;
+        if (tc.group != seen) {
+          named_bar_sync(2, 256);                         // everybody has read the last group's
+          if (tid < kGemvSelfTokens) s_top[tid] = 0;
+          named_bar_sync(2, 256);
+          gemv_with_loader(p, [&](auto load) {
+            next = load_item(load, me);
+            for (int i0 = me; i0 < items; i0 += 32) {
+              Raw8 r[4];
+              #pragma unroll
+              for (int u = 0; u < 4; ++u) r[u] = load_item(load, i0 + 8 * u);
+              #pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (i0 + 8 * u >= items) break;
+                const uint32_t top = __reduce_max_sync(0xffffffffu, largest8(r[u], p.x_dtype));
+                if (lane == 0) atomicMax(&s_top[(i0 + 8 * u) % tc.rows], top);
+              }
+            }
+          });
+          named_bar_sync(2, 256);
+          seen = tc.group;
+        } else {
+          gemv_with_loader(p, [&](auto load) { next = load_item(load, me); });
+        }
+        if (tid < tc.rows) s_back[index % kGemvAhead][tid] = exp2_int(-gemv_exponent(s_top[tid]));
+        __syncwarp();
+        for (int i0 = 0; i0 < items && ok; i0 += 8) {
+          const int i = i0 + me, tok = i % tc.rows;
+          const int c = done + i / tc.rows, slot = c & slot_mask;
+          const Raw8 raw = next;
+          if (i0 + 8 < items) gemv_with_loader(p, [&](auto load) { next = load_item(load, i + 8); });
+          bool free = true;
+          if (i < items) {                                // the same for the whole warp
+            free = ctl.wait(smem_u32(&bar_x_free[slot]), (uint32_t)((c >> slot_bits) & 1) ^ 1u, kDevTimeoutStageFree);
+            free = __all_sync(0xffffffffu, free);
+            if (free) {
+              uint8_t* const image = smem_raw + (x_base - smem_u32(smem_raw)) + slot * x_bytes;
+              float v[8];
+              widen8(raw, p.x_dtype, v);
+              gemv_put(v, exp2_int(gemv_exponent(s_top[tok])), image + tok * kGemvTokenBytes,
+                       image + p.group_rows * kGemvTokenBytes, tok);
+              fence_proxy_async_smem();
+              __syncwarp();
+              // the barrier counts group_rows arrivals: the last row makes up for those that the group lacks
+              if (lane == 0)
+                mbar_arrive_n(smem_u32(&bar_x_full[slot]), tok == tc.rows - 1 ? p.group_rows - tc.rows + 1 : 1);
+            }
+          }
+          ok = !named_bar_any(2, 256, !free);
+        }
+      }
+    } else if (elect_one()) {
+      // ---------------------------------------------------------- x: copied
       const uint64_t pol = policy_evict_normal();
       const int rows_all = kMoe ? p.pairs : p.l * p.m, groups_all = kMoe ? p.pairs : p.l * p.passes;
       int slot = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
       for (int t = cluster; t < tiles && ok; t += clusters) {
-        const GemvTile tc = gemv_tile<kMoe>(p, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
         const uint32_t bytes = tc.rows * kGemvTokenBytes + kGemvXSfBytes;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ctl.wait(smem_u32(&bar_x_free[slot]), phase ^ 1u, kDevTimeoutStageFree)) {
@@ -487,121 +718,145 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const __grid_constan
         for (int s = 0; s < p.x_slots; ++s)
           if ((issued >> s) & 1u) ctl.drain_copies(smem_u32(&bar_x_full[s]), (last_phase >> s) & 1u);
     }
-  } else if (warp == 6) {
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMA
+    // Two issuing threads, each with its own accumulator: an instruction or a
+    // barrier check costs its thread 30 to 100 cycles, and one thread's 770 cycles for a
+    // K block (two waits, eight copies, four MMAs, two commits; measured) were as long as
+    // the block takes to arrive.  They take the weight slots in turn: gate and up, or even and
+    // odd K blocks, whose sums the epilogue adds.  (The number of slots is even, so that a
+    // slot is always the same thread's and its phases are waited for one after the other.)
     if (elect_one()) {
+      const int me = warp - kMmaWarp;
       const uint64_t w_desc0 = kmajor_sw128_desc(w_base), x_desc0 = kmajor_sw128_desc(x_base);
       const uint64_t sf_desc0 = sf_atom_desc(w_base + kBM * kBK / 2), xsf_desc0 = sf_atom_desc(x_base);
-      // accumulators, then each slot's scales: 16 columns for a weight slot, 16 for an x slot
-      const uint32_t sf_col = tmem + kMats * n_pad, xsf_col = sf_col + 16 * p.w_slots;
-      int ws = 0, xs = 0;
+      // accumulators, then for each weight slot 16 columns of its scales and 16 of x's with them (free
+      // when the slot is: the MMAs that read them are done)
+      const uint32_t sf_col = tmem + p.acc_bufs * 2 * n_pad;
+      const int span = kb1 - kb0;
+      int ws = me, xs = kDual ? 0 : me, acc = 0, done = 0;   // done: K blocks before this tile
       uint32_t w_phase = 0, x_phase = 0, acc_phase = 0;
       bool ok = true, any = false;
-      for (int t = cluster; t < tiles && ok; t += clusters) {
-        const GemvTile tc = gemv_tile<kMoe>(p, t);
+      for (int t = cluster; t < tiles && ok; t += clusters, done += span) {
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
         const int n_cols = (tc.rows * kGemvTerms + 15) / 16 * 16;
+        const int xsf_at = (kSelf ? p.group_rows : tc.rows) * kGemvTokenBytes;
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(n_cols >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-        if (!ctl.wait(smem_u32(&bar_acc_free), acc_phase ^ 1u, kDevTimeoutAccFree)) break;
+        const uint32_t d_acc = tmem + (acc * 2 + me) * n_pad;
+        if (!ctl.wait(smem_u32(&bar_acc_free[acc]), acc_phase ^ 1u, kDevTimeoutAccFree)) break;
         tc_fence_after();
-        for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          const int atoms = min(kBK / kKStep, atoms_all - kb * (kBK / kKStep));
-          if (!ctl.wait(smem_u32(&bar_x_full[xs]), x_phase, kDevTimeoutTmaFull)) {
+        uint32_t more = 0;
+        for (int kb = kb0 + (kDual ? 0 : (done ^ me) & 1); kb < kb1; kb += kDual ? 1 : 2) {
+          if (!ctl.wait(smem_u32(&bar_x_full[xs]), x_phase, kDevTimeoutTmaFull) ||
+              !ctl.wait(smem_u32(&bar_w_full[ws]), w_phase, kDevTimeoutTmaFull)) {
             ok = false;
             break;
           }
-          const uint64_t dx = desc_advance(x_desc0, xs * x_bytes);
-          const uint64_t dxs = desc_advance(xsf_desc0, xs * x_bytes + tc.rows * kGemvTokenBytes);
-          const uint32_t xsf = xsf_col + 16 * xs;
+          tc_fence_after();
+          const uint64_t dx = desc_advance(x_desc0, xs * x_bytes), dw = desc_advance(w_desc0, ws * kGemvWBytes);
+          const uint64_t dxs = desc_advance(xsf_desc0, xs * x_bytes + xsf_at);
+          const uint64_t dws = desc_advance(sf_desc0, ws * kGemvWBytes);
+          const uint32_t sf = sf_col + kGemvSfCols * ws, xsf = sf + kGemvSfCols / 2;
+          const int atoms = atoms_all - kb * (kBK / kKStep);
           #pragma unroll
-          for (int mat = 0; mat < kMats; ++mat) {
-            if (!ctl.wait(smem_u32(&bar_w_full[ws]), w_phase, kDevTimeoutTmaFull)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint64_t dw = desc_advance(w_desc0, ws * kGemvWBytes), dws = desc_advance(sf_desc0, ws * kGemvWBytes);
-            const uint32_t sf = sf_col + 16 * ws;
-            for (int j = 0; j < atoms; ++j) {
-              if (mat == 0) tc_cp_32x128b_x4(xsf + 4 * j, desc_advance(dxs, j * kSfAtom));
+          for (int j = 0; j < kBK / kKStep; ++j) {
+            if (j < atoms) {
+              tc_cp_32x128b_x4(xsf + 4 * j, desc_advance(dxs, j * kSfAtom));
               tc_cp_32x128b_x4(sf + 4 * j, desc_advance(dws, j * kSfAtom));
-              tc_mma_nvf4(tmem + mat * n_pad, desc_advance(dw, 32 * j), desc_advance(dx, 32 * j), idesc, sf + 4 * j,
-                          xsf + 4 * j, kb != kb0 || j != 0);
+              tc_mma_nvf4(d_acc, desc_advance(dw, 32 * j), desc_advance(dx, 32 * j), idesc, sf + 4 * j, xsf + 4 * j, more);
+              more = 1;
             }
-            tc_commit(smem_u32(&bar_w_free[ws]));
-            any = true;
-            if (++ws == p.w_slots) ws = 0, w_phase ^= 1u;
           }
-          if (!ok) break;
+          tc_commit(smem_u32(&bar_w_free[ws]));
           tc_commit(smem_u32(&bar_x_free[xs]));
-          if (++xs == p.x_slots) xs = 0, x_phase ^= 1u;
+          any = true;
+          if ((ws += 2) >= p.w_slots) ws -= p.w_slots, w_phase ^= 1u;
+          if ((xs += kDual ? 1 : 2) >= p.x_slots) xs -= p.x_slots, x_phase ^= 1u;
         }
         if (!ok) break;
-        tc_commit(smem_u32(&bar_acc_full));
-        acc_phase ^= 1u;
+        tc_commit(smem_u32(&bar_acc_full[acc]));
+        if (++acc == p.acc_bufs) acc = 0, acc_phase ^= 1u;
       }
       if (s_abort && any) {
-        tc_commit(smem_u32(&bar_drain));
-        ctl.drain(smem_u32(&bar_drain), 0);
+        tc_commit(smem_u32(&bar_drain[me]));
+        ctl.drain(smem_u32(&bar_drain[me]), 0);
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    griddep_wait();                                       // the expansion's factors; and nothing is written before
-    const int lane = (int)(threadIdx.x & 31u), row = warp * 32 + lane;
+    griddep_wait();                                       // nothing is written before
+    const int row = warp * 32 + lane;
     const int own_rows = kBM / splits, owner = row / own_rows;   // the CTA that finishes this thread's row
-    uint32_t phase = 0;
-    for (int t = cluster; t < tiles; t += clusters) {
-      const GemvTile tc = gemv_tile<kMoe>(p, t);
-      if (!ctl.wait(smem_u32(&bar_acc_full), phase, kDevTimeoutAccFull)) break;
+    if constexpr (kMoe && kSelf) {                        // rows without an expert are zero
+      for (int i = (int)blockIdx.x; i < p.pairs; i += (int)gridDim.x)
+        if ((unsigned)__ldg(p.ids + i) >= (unsigned)p.experts)
+          for (int c = row; c < p.n; c += 128) store_out(p.out, p.out_dtype, (int64_t)i * p.ldo + c, 0.f);
+    }
+    uint32_t phase = 0, acc_phase = 0;
+    int acc_buf = 0, index = 0;
+    for (int t = cluster; t < tiles; t += clusters, ++index) {
+      const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+      bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
+      if (splits > 1 && t != cluster)
+        ok = ok && ctl.wait_cluster(smem_u32(&bar_sums_free), phase ^ 1u, kDevTimeoutPeers);
+      if (named_bar_any(1, 128, !ok)) break;              // all of the epilogue's warps or none
       tc_fence_after();
-      if (splits > 1 && t != cluster &&
-          !ctl.wait_cluster(smem_u32(&bar_sums_free), phase ^ 1u, kDevTimeoutAccFree)) break;
-      const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16);
+      const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + acc_buf * 2 * n_pad;
+      // one K block: only the thread whose turn it was has written its accumulator
+      const bool both = kDual || kb1 - kb0 > 1;
+      const int only = index * (kb1 - kb0) & 1;
       // sums of a sender in an owner's shared memory: [sender][matrix][token][row of the owner]
       const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + row % own_rows) * 4u;
       const uint32_t remote = splits > 1 ? mapa_shared(slice, (uint32_t)owner) : 0u;
+      const uint32_t remote_bar = splits > 1 ? mapa_shared(smem_u32(&bar_sums), (uint32_t)owner) : 0u;
+      if (splits > 1 && threadIdx.x == 0)                 // every CTA's sums of this CTA's rows
+        mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * tc.rows * kBM) * 4u);
       auto out_at = [&](int tok) -> int64_t {              // where the token's row of this tile starts
-        const int64_t at = kMoe ? (int64_t)__ldcg(&p.groups->pair[tc.before + tok]) * p.ldo
-                                : (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
+        int64_t at;
+        if constexpr (kMoe) at = (int64_t)(kSelf ? s_small.pair[tc.group][tok] : __ldcg(&p.groups->pair[tc.before + tok])) * p.ldo;
+        else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
         return at + (int64_t)tc.row_block * kBM;
       };
       for (int t0 = 0; t0 < tc.rows; t0 += 2) {
-        uint32_t d[kMats][16];
-        #pragma unroll
-        for (int mat = 0; mat < kMats; ++mat) tmem_ld_32x32b_x16(acc + mat * n_pad + t0 * kGemvTerms, d[mat]);
+        uint32_t d[2][16];
+        tmem_ld_32x32b_x16(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
+        if (both) tmem_ld_32x32b_x16(acc + n_pad + t0 * kGemvTerms, d[1]);
         tmem_ld_wait();
-        #pragma unroll
-        for (int mat = 0; mat < kMats; ++mat) tmem_regs_ready16(d[mat]);
+        tmem_regs_ready16(d[0]), tmem_regs_ready16(d[1]);
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int tok = t0 + i;
           if (tok >= tc.rows) break;
-          const float back = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + tok) * splits + rank);
-          float v[kMats];
+          float back;
+          if constexpr (kSelf) back = s_back[index % kGemvAhead][tok];
+          else back = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + tok) * splits + rank);
+          float v[2] = {0.f, 0.f};
           #pragma unroll
-          for (int mat = 0; mat < kMats; ++mat) {
-            v[mat] = __uint_as_float(d[mat][8 * i + 7]);
-            #pragma unroll
-            for (int j = 6; j >= 0; --j) v[mat] = fmaf(v[mat], 0.125f, __uint_as_float(d[mat][8 * i + j]));
-            v[mat] *= back;
-          }
+          for (int a = 0; a < 2; ++a)
+            if (a == 0 || both) {
+              v[a] = __uint_as_float(d[a][8 * i + 7]);
+              #pragma unroll
+              for (int j = 6; j >= 0; --j) v[a] = fmaf(v[a], 0.125f, __uint_as_float(d[a][8 * i + j]));
+              v[a] *= back;
+            }
+          if constexpr (!kDual) v[0] += v[1];
           if (splits > 1) {
             #pragma unroll
             for (int mat = 0; mat < kMats; ++mat)
-              st_shared_cluster_f32(remote + (uint32_t)((mat * tc.rows + tok) * own_rows) * 4u, v[mat]);
+              st_async_f32(remote + (uint32_t)((mat * tc.rows + tok) * own_rows) * 4u, v[mat], remote_bar);
           } else if (tc.row_block * kBM + row < p.n) {
-            store_out(p.out, p.out_dtype, out_at(tok) + row, kDual ? silu_gate_f32(v[0], v[kMats - 1]) : v[0]);
+            store_out(p.out, p.out_dtype, out_at(tok) + row, kDual ? silu_gate_f32(v[0], v[1]) : v[0]);
           }
         }
       }
       // the accumulators may be overwritten
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free));
+      if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[acc_buf]));
+      if (++acc_buf == p.acc_bufs) acc_buf = 0, acc_phase ^= 1u;
       if (splits > 1) {
-        named_bar_sync(1, 128);
-        if ((int)threadIdx.x < splits) mbar_arrive_cluster(mapa_shared(smem_u32(&bar_sums), threadIdx.x));
-        if (!ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutAccFull)) break;
+        ok = ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutPeers);
+        if (named_bar_any(1, 128, !ok)) break;
         for (int i = (int)threadIdx.x; i < own_rows * tc.rows; i += 128) {
           const int r = i % own_rows, tok = i / own_rows;
           float v[kMats];
@@ -615,17 +870,24 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_kernel(const __grid_constan
           if (tc.row_block * kBM + at < p.n)
             store_out(p.out, p.out_dtype, out_at(tok) + at, kDual ? silu_gate_f32(v[0], v[kMats - 1]) : v[0]);
         }
-        named_bar_sync(1, 128);                           // all of this CTA's rows are read
-        if ((int)threadIdx.x < splits) mbar_arrive_cluster(mapa_shared(smem_u32(&bar_sums_free), threadIdx.x));
+        if (t + clusters < tiles) {
+          named_bar_sync(1, 128);                         // all of this CTA's rows are read: the next may come
+          if ((int)threadIdx.x < splits) mbar_arrive_cluster(mapa_shared(smem_u32(&bar_sums_free), threadIdx.x));
+        }
+        phase ^= 1u;
       }
-      phase ^= 1u;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (splits > 1) cluster_sync();                         // nobody writes to a CTA that is gone
+  // Nobody writes to a CTA that is gone: each has waited for all that the others
+  // send it, unless it gave up a wait.
+  if (splits > 1) {
+    cluster_arrive();
+    if (s_abort) cluster_wait();
+  }
   tc_fence_after();
-  if (warp == 6) tmem_dealloc<kTmemCols>(tmem);
+  if (warp == kMmaWarp) tmem_dealloc<kTmemCols>(tmem);
 }
 
 }  // namespace nvfp4

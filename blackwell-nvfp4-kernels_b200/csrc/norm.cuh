@@ -55,8 +55,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
   return r;
 }
 
-struct Raw8 { uint4 a, b; };           // eight elements as they lie in memory (b: fp32 only)
-
 template <bool kVec>
 __device__ __forceinline__ Raw8 norm_load8(const void* base, int dtype, int64_t at, int left) {
   Raw8 r;
@@ -87,24 +85,6 @@ __device__ __forceinline__ Raw8 norm_load8(const void* base, int dtype, int64_t 
   return r;
 }
 
-__device__ __forceinline__ void norm_widen(const Raw8& r, int dtype, float (&f)[8]) {
-  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-  if (dtype == kDtF32) {
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
-  } else if (dtype == kDtBF16) {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = t.x, f[2 * i + 1] = t.y;
-    }
-  }
-}
-
 // fp32 -> the type's bits; `f` becomes the rounded values.
 __device__ __forceinline__ Raw8 norm_round(float (&f)[8], int dtype) {
   Raw8 r;
@@ -127,7 +107,7 @@ __device__ __forceinline__ Raw8 norm_round(float (&f)[8], int dtype) {
     }
   }
   r.a = make_uint4(h[0], h[1], h[2], h[3]), r.b = make_uint4(0, 0, 0, 0);
-  norm_widen(r, dtype, f);
+  widen8(r, dtype, f);
   return r;
 }
 
@@ -196,7 +176,7 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
   for (int i = 0; i < NV; ++i) {
     const int col = (tid + i * (int)blockDim.x) * 8;
     const Raw8 rx = norm_load8<kVec>(p.x, p.x_dtype, (int64_t)row * p.ldx + col, p.k - col);
-    norm_widen(rx, p.x_dtype, v[i]);
+    widen8(rx, p.x_dtype, v[i]);
     wt[i] = norm_load8<kVec>(p.weight, p.w_dtype, col, p.k - col);
   }
   if (p.residual != nullptr) {
@@ -205,7 +185,7 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
       const int col = (tid + i * (int)blockDim.x) * 8;
       const Raw8 rr = norm_load8<kVec>(p.residual, p.r_dtype, (int64_t)row * p.ldr + col, p.k - col);
       float f[8];
-      norm_widen(rr, p.r_dtype, f);
+      widen8(rr, p.r_dtype, f);
       #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(v[i][e], f[e]);
       const Raw8 h = norm_round(v[i], p.r_dtype);
@@ -233,7 +213,7 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
   #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float w[8];
-    norm_widen(wt[i], p.w_dtype, w);
+    widen8(wt[i], p.w_dtype, w);
     #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], r), w[e]);
   }
