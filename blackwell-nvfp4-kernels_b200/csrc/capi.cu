@@ -1207,8 +1207,6 @@ extern "C" int nvfp4_dual_gemm_noalloc(const void* a, const void* b1, const void
 namespace nvfp4 {
 namespace {
 
-// Half of an SM's shared memory, less what a CTA has besides.
-constexpr int kGemvSmem = 112 * 1024;
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -1239,6 +1237,15 @@ int gemv_splits(long long tiles, int k_blocks, int num_sms) {
     if (s == 1 || load < least) best = s, least = load;
   }
   return best;
+}
+
+// Whether gemv_kernel expands x itself: one launch less, but its eight warps
+// take about 1 us for 8 K blocks of a token.  Measured, us with / without: one token 512 x
+// 1024 4.6 / 5.4, 4096 x 14336 (14 K blocks a CTA) 10.9 / 11.5, 16384 x 7168 (28) 14.6 / 15.3; four
+// tokens 14336 x 4096 (16) 21 / 12.3.  8 experts of one token 4096 x 1536 7.1 / 9.9.
+bool gemv_expands_itself(const GemvParams& p, bool moe, int span) {
+  if (p.x_dtype == kDtF32 || !p.x_vec) return false;
+  return moe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens && p.m * span <= 32;
 }
 
 template <class Kern>
@@ -1292,18 +1299,16 @@ template <bool kDual, bool kMoe>
 int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream) {
   const Knobs kn = read_knobs();
   t_pdl = kn.pdl;
+  constexpr int kMats = kDual ? 2 : 1;
   p.k_blocks = (p.k + kBK - 1) / kBK;
   p.row_blocks = (p.n + kBM - 1) / kBM;
   p.passes = (p.m + kGemvTokens - 1) / kGemvTokens;
   const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
   const long long tiles = (long long)groups * p.row_blocks;
   p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms);
-  if (getenv("GEMV_S")) p.splits = atoi(getenv("GEMV_S"));
-  while (p.splits > p.k_blocks) p.splits /= 2;
   const int span = (p.k_blocks + p.splits - 1) / p.splits;
-  bool self = kMoe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens && p.m * span <= 16;
-  if (getenv("GEMV_SELF")) self = (kMoe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens) && atoi(getenv("GEMV_SELF"));
-  p.room = self ? (kMoe ? 2 : kGemvSelfTokens) : kGemvTokens;
+  const bool self = gemv_expands_itself(p, kMoe, span);
+  p.room = self ? kGemvSelfTokens : kGemvTokens;
   // experts: twice the average of an expert's rows, so that the x slots are not sized for what hardly ever comes
   if (kMoe && !self)
     while (p.room > 4 && (long long)p.room * p.experts >= 4LL * p.pairs) p.room /= 2;
@@ -1315,23 +1320,24 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.image = ws + sp.image;
   p.status = d->status;
   p.wait_limit = wait_limit_cycles();
-  constexpr int kMats = kDual ? 2 : 1;
+  // Shared memory.  Clusters of 8 CTAs find room for all of their SMs only when two
+  // CTAs fit on one (2048 x 7168: 6.8 us with 112 KB, 12.7 with 160).  Otherwise more weight slots pay:
+  // one token 16384 x 7168, 14.6 us with 6 slots, 17.2 with 4; with more than 8 tokens, or
+  // many experts, the x slots need the rest (16 tokens 7168 x 16384 23.6 us with 216 KB, 25.8 with 160).
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
-  const int n_pad = (p.group_rows * kGemvTerms + 15) / 16 * 16;
   const int sums = p.splits > 1 ? kMats * p.group_rows * kBM * (int)sizeof(float) : 0;
-  int budget = p.group_rows > 8 ? 216 * 1024 : kGemvSmem;
-  if (getenv("GEMV_B")) budget = atoi(getenv("GEMV_B")) * 1024;
-  p.x_slots = self ? (p.group_rows <= 2 ? 8 : 4) : 4;
-  if (getenv("GEMV_X") && !self) p.x_slots = atoi(getenv("GEMV_X"));
+  const int budget = (p.splits == 8 && p.group_rows <= 8 ? 112 : p.group_rows > 8 || (kMoe && !self) ? 216 : 160) * 1024;
+  p.x_slots = self ? kGemvMaxXSlots : 4;
   p.w_slots = (budget - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
   if (p.w_slots > kGemvMaxWSlots) p.w_slots = kGemvMaxWSlots;
+  if (self && p.w_slots > 6) p.w_slots = 6;             // TMEM: 256 columns
   p.w_slots &= ~1;
   const int smem = 1024 + p.w_slots * kGemvWBytes + p.x_slots * x_bytes + sums;
   // TMEM: two accumulators (twice where there is room) and the slots' scales
-  const int sf_cols = kGemvSfCols * p.w_slots;
+  const int n_pad = (p.group_rows * kGemvTerms + 15) / 16 * 16, sf_cols = kGemvSfCols * p.w_slots;
   p.acc_bufs = 4 * n_pad + sf_cols <= 256 ? 2 : 2 * n_pad + sf_cols <= 256 ? 1 : 4 * n_pad + sf_cols <= 512 ? 2 : 1;
   const int cols = p.acc_bufs * 2 * n_pad + sf_cols;
-  if (p.w_slots < 2 || cols > (self ? 256 : 512))
+  if (p.w_slots < 2 || cols > (self ? 256 : 512) || (self && p.acc_bufs != 2))
     return fail(NVFP4_ERR_SHAPE, "%d weight slots, %d TMEM columns", p.w_slots, cols);
   const int base = 32 + (kDual ? 6 : 0) + (kMoe ? 3 : 0);
   if (self) return launch_gemv<kDual, kMoe, true, 256>(d, base, p, smem, tiles, stream);

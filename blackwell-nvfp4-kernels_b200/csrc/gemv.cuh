@@ -123,6 +123,11 @@ constexpr int kExpandBlocks = kExpandThreads / 32;        // K blocks of a CTA
 
 // Eight consecutive elements as they lie in memory (b: fp32 only).  kVec: 16-byte aligned.
 struct Raw8 { uint4 a, b; };
+__device__ __forceinline__ uint4 ldg_v4(const void* q) {   // volatile: stays in front of a signal that follows it
+  uint4 v;
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(q));
+  return v;
+}
 template <bool kWide, bool kVec>
 __device__ __forceinline__ Raw8 gemv_raw8(const void* x, int64_t at) {
   Raw8 r;
@@ -130,7 +135,7 @@ __device__ __forceinline__ Raw8 gemv_raw8(const void* x, int64_t at) {
   if constexpr (kWide) {
     const uint32_t* q = static_cast<const uint32_t*>(x) + at;
     if constexpr (kVec) {
-      r.a = __ldg(reinterpret_cast<const uint4*>(q)), r.b = __ldg(reinterpret_cast<const uint4*>(q) + 1);
+      r.a = ldg_v4(q), r.b = ldg_v4(q + 4);
     } else {
       r.a = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
       r.b = make_uint4(__ldg(q + 4), __ldg(q + 5), __ldg(q + 6), __ldg(q + 7));
@@ -138,7 +143,7 @@ __device__ __forceinline__ Raw8 gemv_raw8(const void* x, int64_t at) {
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(x) + at;
     if constexpr (kVec) {
-      r.a = __ldg(reinterpret_cast<const uint4*>(q));
+      r.a = ldg_v4(q);
     } else {
       uint32_t v[4];
       #pragma unroll
@@ -405,26 +410,15 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
 constexpr int kGemvWBytes = kBM * kBK / 2 + kSfStageBytes;   // a weight slot: 128 rows x 256, scale atoms
 constexpr int kGemvSfCols = 32;          // TMEM columns of a weight slot: its scales and x's
 constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // x slots a power of two
-constexpr int kGemvSelfTokens = 4;       // largest group that gemv_kernel expands itself
-// tiles that the expansion may be ahead of the epilogue: two accumulators, x slots of one K block each
-constexpr int kGemvAhead = kGemvMaxXSlots + 4;
+constexpr int kGemvSelfTokens = 2;       // largest group that gemv_kernel expands itself
+constexpr int kGemvAhead = 2;            // the expansion is at most a tile ahead of the epilogue
 constexpr int kGemvSelfPairs = 32;       // and the most rows of an expert call
-// warps: epilogue 0-3, expansion 4-11 (without it x copies: 4), then weights, two for the MMAs
-constexpr int gemv_threads(bool self) { return 32 * (self ? 15 : 8); }
+// warps: epilogue 0-3, expansion 0-7 (without it x copies: 4), then weights, two for the MMAs
+constexpr int gemv_threads(bool self) { return 32 * (self ? 11 : 8); }
 
 // Copy one scale atom into TMEM: row i to lane i of each lane quadrant, 4 columns.
 __device__ __forceinline__ void tc_cp_32x128b_x4(uint32_t taddr, uint64_t s_desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
-}
-
-// Hints: bring a weight slot's bytes into L2.
-__device__ __forceinline__ void prefetch_l2_3d(const void* tmap, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tmap), "r"(c0), "r"(c1),
-               "r"(c2)
-               : "memory");
-}
-__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
 // Store to shared memory of any CTA of the cluster, its bytes counted on an
@@ -471,18 +465,17 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSma
 
 // A cluster of `splits` CTAs owns a 128-row block and a group; each CTA has a
 // part of K.  Shared memory holds a ring of weight slots (one matrix' K block,
-// 18 KB) and a ring of x slots; it is kept to half of the SM's, so that the next
-// kernel's CTAs can be resident and get ready while this one ends.  The sums of
-// the CTAs of a cluster meet in distributed shared memory: each CTA owns 128 / splits rows,
-// gets the others' sums for them and adds them in the order of the CTAs.
+// 18 KB) and a ring of x slots.  The sums of the CTAs of a cluster meet in distributed
+// shared memory: each CTA owns 128 / splits rows, gets the others' sums for them and
+// adds them in the order of the CTAs.
 template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
-__global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_constant__ GemvParams p) {
+__global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __grid_constant__ GemvParams p) {
   constexpr int kMats = kDual ? 2 : 1;
-  constexpr int kWWarp = kSelf ? 12 : 5, kMmaWarp = kWWarp + 1;   // and kMmaWarp + 1
+  constexpr int kWWarp = kSelf ? 8 : 5, kMmaWarp = kWWarp + 1;   // and kMmaWarp + 1
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_w_full[kGemvMaxWSlots], bar_w_free[kGemvMaxWSlots];
   __shared__ uint64_t bar_x_full[kGemvMaxXSlots], bar_x_free[kGemvMaxXSlots];
-  __shared__ uint64_t bar_acc_full[2], bar_acc_free[2], bar_drain[2];
+  __shared__ uint64_t bar_acc_full[2], bar_acc_free[2], bar_drain[2], bar_go;
   __shared__ uint64_t bar_sums, bar_sums_free;            // this CTA's rows: all sums there; its sums taken everywhere
   __shared__ uint32_t s_tmem_base;
   __shared__ volatile int s_abort;
@@ -515,8 +508,10 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
       mbar_init(smem_u32(&bar_drain[i]), 1);
     }
     mbar_init(smem_u32(&bar_sums), 1);
+    mbar_init(smem_u32(&bar_go), 8);
     mbar_init(smem_u32(&bar_sums_free), splits);
     s_abort = 0;
+    for (int i = 0; i < kGemvSelfTokens; ++i) s_top[i] = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
@@ -558,23 +553,10 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
       int slot = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
-      if constexpr (kSelf && !kMoe) {
-        // the first slots' bytes towards L2 while earlier kernels end (they may still write them: a
-        // prefetch is only a hint, and L2 is where everybody sees them), the loads after the wait
-        if (cluster < tiles) {
-          const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, cluster);
-          const size_t atom0 = ((size_t)tc.batch * p.row_blocks + tc.row_block) * (size_t)atoms_all;
-          for (int kb = kb0; kb < min(kb1, kb0 + p.w_slots / kMats); ++kb) {
-            const int atoms = min(kBK / kKStep, atoms_all - kb * (kBK / kKStep));
-            prefetch_l2_3d(&p.map1, kb * (kBK / 2), tc.row_block * kBM, tc.batch);
-            prefetch_l2(p.sf1 + (atom0 + (size_t)kb * (kBK / kKStep)) * kSfAtom, atoms * kSfAtom);
-            if constexpr (kDual) {
-              prefetch_l2_3d(&p.map2, kb * (kBK / 2), tc.row_block * kBM, tc.batch);
-              prefetch_l2(p.sf2 + (atom0 + (size_t)kb * (kBK / kKStep)) * kSfAtom, atoms * kSfAtom);
-            }
-          }
-        }
+      if constexpr (kSelf) {
+        // x's loads first: behind the weights' first slots they would take twice as long
         griddep_wait();
+        if (cluster < tiles) ctl.wait(smem_u32(&bar_go), 0, kDevTimeoutStageFree);
       }
       for (int t = cluster; t < tiles && ok; t += clusters) {
         const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
@@ -589,6 +571,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
           const int atoms = min(kBK / kKStep, atoms_all - kb * (kBK / kKStep));
           #pragma unroll
           for (int mat = 0; mat < kMats; ++mat) {
+            if (!kSelf && !kMoe && slot == 0 && phase == 1u) griddep_wait();   // the ring is full: again, no polling
             if (!ctl.wait(smem_u32(&bar_w_free[slot]), phase ^ 1u, kDevTimeoutStageFree)) {
               ok = false;
               break;
@@ -608,90 +591,10 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
         for (int s = 0; s < p.w_slots; ++s)
           if ((issued >> s) & 1u) ctl.drain_copies(smem_u32(&bar_w_full[s]), (last_phase >> s) & 1u);
     }
-  } else if (warp >= 4 && warp < kWWarp) {
-    griddep_wait();                                       // x, or the expansion of it
-    if constexpr (kSelf) {
-      // ---------------------------------------------------------- x: expanded here
-      // a warp takes one token's K block at a time, a lane 8 elements; 8 of them a
-      // round.  The warps end each round together: a slot's next user then cannot wait for
-      // its barrier before this round's user has (the parity of a phase says nothing
-      // about the phase two before), and all give up if one has to.
-      const int me = warp - 4, tid = (int)threadIdx.x - 128;
-      const int span = kb1 - kb0;
-      const int slot_mask = p.x_slots - 1, slot_bits = __popc(slot_mask);
-      int seen = -1, done = 0, index = 0;                 // group whose s_top is there; K blocks before this tile
-      bool ok = true;
-      for (int t = cluster; t < tiles && ok; t += clusters, done += span, ++index) {
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
-        auto x_at = [&](int tok) -> int64_t {
-          if constexpr (kMoe) {
-            const int pr = s_small.pair[tc.group][tok];
-            return (int64_t)(p.x_per_pair ? pr : pr / p.topk) * p.ldx;
-          }
-          return (int64_t)tc.batch * p.x_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldx;
-        };
-        const int items = span * tc.rows;
-        // an item's elements, loaded a round ahead
-        auto load_item = [&](auto load, int i) {
-          const int k0 = (kb0 + i / tc.rows) * kBK + lane * 8, tok = i % tc.rows;
-          Raw8 r;
-          r.a = r.b = make_uint4(0, 0, 0, 0);
-          if (i < items && k0 < p.k) r = load(x_at(tok) + k0);
-          return r;
-        };
-        Raw8 next;
-        if (tc.group != seen) {
-          named_bar_sync(2, 256);                         // everybody has read the last group's
-          if (tid < kGemvSelfTokens) s_top[tid] = 0;
-          named_bar_sync(2, 256);
-          gemv_with_loader(p, [&](auto load) {
-            next = load_item(load, me);
-            for (int i0 = me; i0 < items; i0 += 32) {
-              Raw8 r[4];
-              #pragma unroll
-              for (int u = 0; u < 4; ++u) r[u] = load_item(load, i0 + 8 * u);
-              #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                if (i0 + 8 * u >= items) break;
-                const uint32_t top = __reduce_max_sync(0xffffffffu, largest8(r[u], p.x_dtype));
-                if (lane == 0) atomicMax(&s_top[(i0 + 8 * u) % tc.rows], top);
-              }
-            }
-          });
-          named_bar_sync(2, 256);
-          seen = tc.group;
-        } else {
-          gemv_with_loader(p, [&](auto load) { next = load_item(load, me); });
-        }
-        if (tid < tc.rows) s_back[index % kGemvAhead][tid] = exp2_int(-gemv_exponent(s_top[tid]));
-        __syncwarp();
-        for (int i0 = 0; i0 < items && ok; i0 += 8) {
-          const int i = i0 + me, tok = i % tc.rows;
-          const int c = done + i / tc.rows, slot = c & slot_mask;
-          const Raw8 raw = next;
-          if (i0 + 8 < items) gemv_with_loader(p, [&](auto load) { next = load_item(load, i + 8); });
-          bool free = true;
-          if (i < items) {                                // the same for the whole warp
-            free = ctl.wait(smem_u32(&bar_x_free[slot]), (uint32_t)((c >> slot_bits) & 1) ^ 1u, kDevTimeoutStageFree);
-            free = __all_sync(0xffffffffu, free);
-            if (free) {
-              uint8_t* const image = smem_raw + (x_base - smem_u32(smem_raw)) + slot * x_bytes;
-              float v[8];
-              widen8(raw, p.x_dtype, v);
-              gemv_put(v, exp2_int(gemv_exponent(s_top[tok])), image + tok * kGemvTokenBytes,
-                       image + p.group_rows * kGemvTokenBytes, tok);
-              fence_proxy_async_smem();
-              __syncwarp();
-              // the barrier counts group_rows arrivals: the last row makes up for those that the group lacks
-              if (lane == 0)
-                mbar_arrive_n(smem_u32(&bar_x_full[slot]), tok == tc.rows - 1 ? p.group_rows - tc.rows + 1 : 1);
-            }
-          }
-          ok = !named_bar_any(2, 256, !free);
-        }
-      }
-    } else if (elect_one()) {
-      // ---------------------------------------------------------- x: copied
+  } else if (!kSelf && warp == 4) {
+    // ------------------------------------------------------------ x: copied
+    griddep_wait();                                       // the expansion is done
+    if (elect_one()) {
       const uint64_t pol = policy_evict_normal();
       const int rows_all = kMoe ? p.pairs : p.l * p.m, groups_all = kMoe ? p.pairs : p.l * p.passes;
       int slot = 0;
@@ -726,6 +629,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
     // the block takes to arrive.  They take the weight slots in turn: gate and up, or even and
     // odd K blocks, whose sums the epilogue adds.  (The number of slots is even, so that a
     // slot is always the same thread's and its phases are waited for one after the other.)
+    griddep_wait();                                       // nothing to do before; and no polling beside a kernel at work
     if (elect_one()) {
       const int me = warp - kMmaWarp;
       const uint64_t w_desc0 = kmajor_sw128_desc(w_base), x_desc0 = kmajor_sw128_desc(x_base);
@@ -783,99 +687,197 @@ __global__ void __launch_bounds__(gemv_threads(kSelf)) gemv_kernel(const __grid_
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue
-    griddep_wait();                                       // nothing is written before
+    // ------------------------------------------------------------ workers: expansion, epilogue
+    griddep_wait();                                       // x or its expansion; and nothing is written before
     const int row = warp * 32 + lane;
     const int own_rows = kBM / splits, owner = row / own_rows;   // the CTA that finishes this thread's row
     if constexpr (kMoe && kSelf) {                        // rows without an expert are zero
       for (int i = (int)blockIdx.x; i < p.pairs; i += (int)gridDim.x)
         if ((unsigned)__ldg(p.ids + i) >= (unsigned)p.experts)
-          for (int c = row; c < p.n; c += 128) store_out(p.out, p.out_dtype, (int64_t)i * p.ldo + c, 0.f);
+          for (int c = row; c < p.n; c += 256) store_out(p.out, p.out_dtype, (int64_t)i * p.ldo + c, 0.f);
     }
-    uint32_t phase = 0, acc_phase = 0;
-    int acc_buf = 0, index = 0;
-    for (int t = cluster; t < tiles; t += clusters, ++index) {
-      const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
-      bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
-      if (splits > 1 && t != cluster)
-        ok = ok && ctl.wait_cluster(smem_u32(&bar_sums_free), phase ^ 1u, kDevTimeoutPeers);
-      if (named_bar_any(1, 128, !ok)) break;              // all of the epilogue's warps or none
-      tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + acc_buf * 2 * n_pad;
-      // one K block: only the thread whose turn it was has written its accumulator
-      const bool both = kDual || kb1 - kb0 > 1;
-      const int only = index * (kb1 - kb0) & 1;
-      // sums of a sender in an owner's shared memory: [sender][matrix][token][row of the owner]
-      const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + row % own_rows) * 4u;
-      const uint32_t remote = splits > 1 ? mapa_shared(slice, (uint32_t)owner) : 0u;
-      const uint32_t remote_bar = splits > 1 ? mapa_shared(smem_u32(&bar_sums), (uint32_t)owner) : 0u;
-      if (splits > 1 && threadIdx.x == 0)                 // every CTA's sums of this CTA's rows
-        mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * tc.rows * kBM) * 4u);
-      auto out_at = [&](int tok) -> int64_t {              // where the token's row of this tile starts
-        int64_t at;
-        if constexpr (kMoe) at = (int64_t)(kSelf ? s_small.pair[tc.group][tok] : __ldcg(&p.groups->pair[tc.before + tok])) * p.ldo;
-        else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
-        return at + (int64_t)tc.row_block * kBM;
-      };
-      for (int t0 = 0; t0 < tc.rows; t0 += 2) {
-        uint32_t d[2][16];
-        tmem_ld_32x32b_x16(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
-        if (both) tmem_ld_32x32b_x16(acc + n_pad + t0 * kGemvTerms, d[1]);
-        tmem_ld_wait();
-        tmem_regs_ready16(d[0]), tmem_regs_ready16(d[1]);
-        #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int tok = t0 + i;
-          if (tok >= tc.rows) break;
-          float back;
-          if constexpr (kSelf) back = s_back[index % kGemvAhead][tok];
-          else back = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + tok) * splits + rank);
-          float v[2] = {0.f, 0.f};
+    // Expansion of a tile's x.  A warp takes one token's K block at a time, a lane
+    // 8 elements; 8 of them a round.  The warps end each round together: a slot's next
+    // user then cannot wait for its barrier before this round's user has (the parity of a
+    // phase says nothing about the phase two before), and all give up if one has to.
+    const int me = warp, tid = (int)threadIdx.x, span = kb1 - kb0;
+    const int slot_mask = p.x_slots - 1, slot_bits = __popc(slot_mask);
+    int seen = -1;                                        // the group whose s_top is there
+    auto expand = [&](int t, int index) -> bool {
+      bool ok = true;
+      if constexpr (kSelf) {                              // x in 16 bits, 16-byte aligned
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        auto x_at = [&](int tok) -> int64_t {
+          if constexpr (kMoe) {
+            const int pr = s_small.pair[tc.group][tok];
+            return (int64_t)(p.x_per_pair ? pr : pr / p.topk) * p.ldx;
+          }
+          return (int64_t)tc.batch * p.x_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldx;
+        };
+        const int items = span * tc.rows, done = index * span;
+        // the elements of four rounds' items at a time
+        auto load_batch = [&](uint4 (&r)[4], int i0) {
           #pragma unroll
-          for (int a = 0; a < 2; ++a)
-            if (a == 0 || both) {
-              v[a] = __uint_as_float(d[a][8 * i + 7]);
-              #pragma unroll
-              for (int j = 6; j >= 0; --j) v[a] = fmaf(v[a], 0.125f, __uint_as_float(d[a][8 * i + j]));
-              v[a] *= back;
-            }
-          if constexpr (!kDual) v[0] += v[1];
-          if (splits > 1) {
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 8 * u + me, k0 = (kb0 + i / tc.rows) * kBK + lane * 8;
+            r[u] = make_uint4(0, 0, 0, 0);
+            if (i < items && k0 < p.k) r[u] = ldg_v4(static_cast<const uint16_t*>(p.x) + x_at(i % tc.rows) + k0);
+          }
+        };
+        uint4 raw[4];
+        load_batch(raw, 0);
+        if (index == 0 && lane == 0) mbar_arrive(smem_u32(&bar_go));
+        if (tc.group != seen) {
+          if (seen >= 0) {
+            named_bar_sync(2, 256);                       // everybody has read the last group's
+            if (tid < kGemvSelfTokens) s_top[tid] = 0;
+            named_bar_sync(2, 256);
+          }
+          auto take = [&](const uint4 (&r)[4], int i0) {
             #pragma unroll
-            for (int mat = 0; mat < kMats; ++mat)
-              st_async_f32(remote + (uint32_t)((mat * tc.rows + tok) * own_rows) * 4u, v[mat], remote_bar);
-          } else if (tc.row_block * kBM + row < p.n) {
-            store_out(p.out, p.out_dtype, out_at(tok) + row, kDual ? silu_gate_f32(v[0], v[1]) : v[0]);
+            for (int u = 0; u < 4; ++u) {
+              const int i = i0 + 8 * u + me;
+              if (i >= items) break;
+              const uint32_t top = __reduce_max_sync(0xffffffffu, largest8(Raw8{r[u], {}}, p.x_dtype));
+              if (lane == 0) atomicMax(&s_top[i % tc.rows], top);
+            }
+          };
+          take(raw, 0);
+          for (int i0 = 32; i0 < items; i0 += 32) {
+            uint4 r[4];
+            load_batch(r, i0);
+            take(r, i0);
           }
+          named_bar_sync(2, 256);
+          seen = tc.group;
         }
-      }
-      // the accumulators may be overwritten
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[acc_buf]));
-      if (++acc_buf == p.acc_bufs) acc_buf = 0, acc_phase ^= 1u;
-      if (splits > 1) {
-        ok = ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutPeers);
-        if (named_bar_any(1, 128, !ok)) break;
-        for (int i = (int)threadIdx.x; i < own_rows * tc.rows; i += 128) {
-          const int r = i % own_rows, tok = i / own_rows;
-          float v[kMats];
+        if (tid < tc.rows) s_back[index % kGemvAhead][tid] = exp2_int(-gemv_exponent(s_top[tid]));
+        __syncwarp();
+        for (int i0 = 0; i0 < items && ok; i0 += 32) {
+          if (i0 > 0) load_batch(raw, i0);
           #pragma unroll
-          for (int mat = 0; mat < kMats; ++mat) {
-            v[mat] = 0.f;
-            for (int s = 0; s < splits; ++s)
-              v[mat] += __uint_as_float(lds_u32(sums_base + (uint32_t)(((s * kMats + mat) * tc.rows + tok) * own_rows + r) * 4u));
+          for (int u = 0; u < 4; ++u) {
+            if (i0 + 8 * u >= items || !ok) break;
+            const int i = i0 + 8 * u + me, tok = i % tc.rows;
+            const int c = done + i / tc.rows, slot = c & slot_mask;
+            bool free = true;
+            if (i < items) {                              // the same for the whole warp
+              free = ctl.wait(smem_u32(&bar_x_free[slot]), (uint32_t)((c >> slot_bits) & 1) ^ 1u, kDevTimeoutStageFree);
+              free = __all_sync(0xffffffffu, free);
+              if (free) {
+                uint8_t* const image = smem_raw + (x_base - smem_u32(smem_raw)) + slot * x_bytes;
+                float v[8];
+                widen8(Raw8{raw[u], {}}, p.x_dtype, v);
+                gemv_put(v, exp2_int(gemv_exponent(s_top[tok])), image + tok * kGemvTokenBytes,
+                         image + p.group_rows * kGemvTokenBytes, tok);
+                fence_proxy_async_smem();
+                __syncwarp();
+                // the barrier counts group_rows arrivals: the last row makes up for those that the group lacks
+                if (lane == 0)
+                  mbar_arrive_n(smem_u32(&bar_x_full[slot]), tok == tc.rows - 1 ? p.group_rows - tc.rows + 1 : 1);
+              }
+            }
+            ok = !named_bar_any(2, 256, !free);
           }
-          const int at = rank * own_rows + r;
-          if (tc.row_block * kBM + at < p.n)
-            store_out(p.out, p.out_dtype, out_at(tok) + at, kDual ? silu_gate_f32(v[0], v[kMats - 1]) : v[0]);
         }
-        if (t + clusters < tiles) {
-          named_bar_sync(1, 128);                         // all of this CTA's rows are read: the next may come
-          if ((int)threadIdx.x < splits) mbar_arrive_cluster(mapa_shared(smem_u32(&bar_sums_free), threadIdx.x));
-        }
-        phase ^= 1u;
       }
+      return ok;
+    };
+    // A tile's sums: from TMEM, over the cluster, to the output.
+    uint32_t phase = 0, acc_phase = 0;
+    int acc_buf = 0;
+    auto finish = [&](int t, int index) -> bool {
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
+        if (splits > 1 && t != cluster)
+          ok = ok && ctl.wait_cluster(smem_u32(&bar_sums_free), phase ^ 1u, kDevTimeoutPeers);
+        if (named_bar_any(1, 128, !ok)) return false;       // all of the epilogue's warps or none
+        tc_fence_after();
+        const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + acc_buf * 2 * n_pad;
+        // one K block: only the thread whose turn it was has written its accumulator
+        const bool both = kDual || kb1 - kb0 > 1;
+        const int only = index * (kb1 - kb0) & 1;
+        // sums of a sender in an owner's shared memory: [sender][matrix][token][row of the owner]
+        const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + row % own_rows) * 4u;
+        const uint32_t remote = splits > 1 ? mapa_shared(slice, (uint32_t)owner) : 0u;
+        const uint32_t remote_bar = splits > 1 ? mapa_shared(smem_u32(&bar_sums), (uint32_t)owner) : 0u;
+        if (splits > 1 && threadIdx.x == 0)                 // every CTA's sums of this CTA's rows
+          mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * tc.rows * kBM) * 4u);
+        auto out_at = [&](int tok) -> int64_t {              // where the token's row of this tile starts
+          int64_t at;
+          if constexpr (kMoe) at = (int64_t)(kSelf ? s_small.pair[tc.group][tok] : __ldcg(&p.groups->pair[tc.before + tok])) * p.ldo;
+          else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
+          return at + (int64_t)tc.row_block * kBM;
+        };
+        for (int t0 = 0; t0 < tc.rows; t0 += 2) {
+          uint32_t d[2][16];
+          tmem_ld_32x32b_x16(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
+          if (both) tmem_ld_32x32b_x16(acc + n_pad + t0 * kGemvTerms, d[1]);
+          tmem_ld_wait();
+          tmem_regs_ready16(d[0]), tmem_regs_ready16(d[1]);
+          #pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int tok = t0 + i;
+            if (tok >= tc.rows) break;
+            float back;
+            if constexpr (kSelf) back = s_back[index % kGemvAhead][tok];
+            else back = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + tok) * splits + rank);
+            float v[2] = {0.f, 0.f};
+            #pragma unroll
+            for (int a = 0; a < 2; ++a)
+              if (a == 0 || both) {
+                v[a] = __uint_as_float(d[a][8 * i + 7]);
+                #pragma unroll
+                for (int j = 6; j >= 0; --j) v[a] = fmaf(v[a], 0.125f, __uint_as_float(d[a][8 * i + j]));
+                v[a] *= back;
+              }
+            if constexpr (!kDual) v[0] += v[1];
+            if (splits > 1) {
+              #pragma unroll
+              for (int mat = 0; mat < kMats; ++mat)
+                st_async_f32(remote + (uint32_t)((mat * tc.rows + tok) * own_rows) * 4u, v[mat], remote_bar);
+            } else if (tc.row_block * kBM + row < p.n) {
+              store_out(p.out, p.out_dtype, out_at(tok) + row, kDual ? silu_gate_f32(v[0], v[1]) : v[0]);
+            }
+          }
+        }
+        // the accumulators may be overwritten
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[acc_buf]));
+        if (++acc_buf == p.acc_bufs) acc_buf = 0, acc_phase ^= 1u;
+        if (splits > 1) {
+          ok = ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutPeers);
+          if (named_bar_any(1, 128, !ok)) return false;
+          for (int i = (int)threadIdx.x; i < own_rows * tc.rows; i += 128) {
+            const int r = i % own_rows, tok = i / own_rows;
+            float v[kMats];
+            #pragma unroll
+            for (int mat = 0; mat < kMats; ++mat) {
+              v[mat] = 0.f;
+              for (int s = 0; s < splits; ++s)
+                v[mat] += __uint_as_float(lds_u32(sums_base + (uint32_t)(((s * kMats + mat) * tc.rows + tok) * own_rows + r) * 4u));
+            }
+            const int at = rank * own_rows + r;
+            if (tc.row_block * kBM + at < p.n)
+              store_out(p.out, p.out_dtype, out_at(tok) + at, kDual ? silu_gate_f32(v[0], v[kMats - 1]) : v[0]);
+          }
+          if (t + clusters < tiles) {
+            named_bar_sync(1, 128);                         // all of this CTA's rows are read: the next may come
+            if ((int)threadIdx.x < splits) mbar_arrive_cluster(mapa_shared(smem_u32(&bar_sums_free), threadIdx.x));
+          }
+          phase ^= 1u;
+        }
+      return true;
+    };
+    // the next tile's x before a tile's end: that has a second accumulator to wait in
+    bool finishing = warp < 4;
+    const int count = cluster < tiles ? (tiles - 1 - cluster) / clusters + 1 : 0;
+    #pragma unroll 1
+    for (int i = 0; i < count + (kSelf ? 1 : 0); ++i) {
+      if (kSelf && i < count && !expand(cluster + i * clusters, i)) break;
+      const int f = kSelf ? i - 1 : i;
+      if (f >= 0 && finishing) finishing = finish(cluster + f * clusters, f);
     }
   }
   tc_fence_before();
