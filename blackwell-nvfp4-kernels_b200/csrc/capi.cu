@@ -1243,9 +1243,26 @@ int gemv_splits(long long tiles, int k_blocks, int num_sms) {
 // take about 1 us for 8 K blocks of a token.  Measured, us with / without: one token 512 x
 // 1024 4.6 / 5.4, 4096 x 14336 (14 K blocks a CTA) 10.9 / 11.5, 16384 x 7168 (28) 14.6 / 15.3; four
 // tokens 14336 x 4096 (16) 21 / 12.3.  8 experts of one token 4096 x 1536 7.1 / 9.9.
-bool gemv_expands_itself(const GemvParams& p, bool moe, int span) {
-  if (p.x_dtype == kDtF32 || !p.x_vec) return false;
-  return moe ? p.pairs <= kGemvSelfPairs : p.m <= kGemvSelfTokens && p.m * span <= 32;
+bool gemv_expands_itself(int x_dtype, bool x_vec, int rows, int span) {
+  return x_dtype != kDtF32 && x_vec && rows <= kGemvSelfTokens && rows * span <= 32;
+}
+bool gemv_expands_itself(int x_dtype, bool x_vec, int pairs) { return x_dtype != kDtF32 && x_vec && pairs <= kGemvSelfPairs; }
+
+// K blocks of a CTA.
+int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
+  const int k_blocks = (k + kBK - 1) / kBK;
+  const long long tiles = (long long)l * ((m + kGemvTokens - 1) / kGemvTokens) * ((n + kBM - 1) / kBM);
+  *splits = gemv_splits(tiles, k_blocks, num_sms);
+  return (k_blocks + *splits - 1) / *splits;
+}
+
+size_t gemv_workspace(int x_dtype, bool x_vec, int m, int n, int k, int l, int num_sms) {
+  int splits;
+  if (gemv_expands_itself(x_dtype, x_vec, m, gemv_span(m, n, k, l, num_sms, &splits))) return 0;
+  return gemv_space(false, (long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
+}
+size_t moe_gemv_workspace(int x_dtype, bool x_vec, int pairs, int k) {
+  return gemv_expands_itself(x_dtype, x_vec, pairs) ? 0 : gemv_space(true, pairs, pairs, k).total;
 }
 
 template <class Kern>
@@ -1307,7 +1324,8 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   const long long tiles = (long long)groups * p.row_blocks;
   p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms);
   const int span = (p.k_blocks + p.splits - 1) / p.splits;
-  const bool self = gemv_expands_itself(p, kMoe, span);
+  const bool self = kMoe ? gemv_expands_itself(p.x_dtype, p.x_vec, p.pairs)
+                         : gemv_expands_itself(p.x_dtype, p.x_vec, p.m, span);
   p.room = self ? kGemvSelfTokens : kGemvTokens;
   // experts: twice the average of an expert's rows, so that the x slots are not sized for what hardly ever comes
   if (kMoe && !self)
@@ -1351,25 +1369,34 @@ bool dtype_ok(int t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
 // Sizes, types and alignment that all the products share.
 constexpr int kGemvMaxRows = 4096;   // rows of x in a batch entry
 
-int validate_gemv(const GemvParams& p, const void* workspace, size_t workspace_bytes, size_t need) {
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (bytes < need || (need > 0 && !workspace))
+    return fail(NVFP4_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", bytes, need);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(NVFP4_ERR_ALIGNMENT, "the workspace must be 256-byte aligned");
+  return NVFP4_OK;
+}
+
+int validate_gemv(const GemvParams& p) {
   if (!dtype_ok(p.x_dtype) || !dtype_ok(p.out_dtype)) return fail(NVFP4_ERR_INVALID_ARG, "bad dtype (x %d, out %d)", p.x_dtype, p.out_dtype);
   if (p.k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", p.k);
   if ((long long)p.n * p.k * p.l >= (1LL << 41) || (long long)p.m * p.l * p.k >= (1LL << 31))
     return fail(NVFP4_ERR_SHAPE, "problem too large");
   if (p.ldx < 0 || p.ldo < p.n) return fail(NVFP4_ERR_INVALID_ARG, "bad row strides (x %lld, out %lld)", (long long)p.ldx, (long long)p.ldo);
-  if (workspace_bytes < need) return fail(NVFP4_ERR_INVALID_ARG, "workspace too small (%zu < %zu bytes)", workspace_bytes, need);
   if ((reinterpret_cast<uintptr_t>(p.x) & (dtype_size(p.x_dtype) - 1)) ||
-      (reinterpret_cast<uintptr_t>(p.out) & (dtype_size(p.out_dtype) - 1)) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
-    return fail(NVFP4_ERR_ALIGNMENT, "x and out must be aligned to their elements, the workspace to 256 bytes");
+      (reinterpret_cast<uintptr_t>(p.out) & (dtype_size(p.out_dtype) - 1)))
+    return fail(NVFP4_ERR_ALIGNMENT, "x and out must be aligned to their elements");
   return NVFP4_OK;
 }
 
 }  // namespace
 }  // namespace nvfp4
 
-extern "C" size_t nvfp4_gemv_workspace_bytes(int m, int k, int l) {
-  if (m < 1 || k < 1 || l < 1) return 0;
-  return gemv_space(false, (long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
+extern "C" size_t nvfp4_gemv_workspace_bytes(int x_dtype, int x_aligned, int m, int n, int k, int l) {
+  if (m < 1 || n < 1 || k < 1 || l < 1) return 0;
+  DeviceState* d = nullptr;
+  if (get_device(&d)) return gemv_workspace(kDtF32, false, m, n, k, l, 1);   // no device: the most it can be
+  return gemv_workspace(x_dtype, x_aligned != 0, m, n, k, l, d->num_sms);
 }
 
 extern "C" int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x_batch, const void* b1,
@@ -1379,7 +1406,7 @@ extern "C" int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x
   if (m < 0 || n < 1 || k < 1 || l < 1)
     return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (m=%d n=%d k=%d l=%d)", m, n, k, l);
   if (m == 0) return NVFP4_OK;
-  if (!x || !b1 || !sf1 || !out || !workspace || !b2 != !sf2) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if (!x || !b1 || !sf1 || !out || !b2 != !sf2) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
   if (m > kGemvMaxRows || l > 4096) return fail(NVFP4_ERR_SHAPE, "%d rows (at most %d), %d batch entries (at most 4096)", m, kGemvMaxRows, l);
   if (!aligned16(b1) || !aligned16(b2) || !aligned16(sf1) || !aligned16(sf2))
     return fail(NVFP4_ERR_ALIGNMENT, "weights and scale atoms must be 16-byte aligned");
@@ -1388,12 +1415,13 @@ extern "C" int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x
   p.x = x, p.ldx = ldx, p.x_batch = x_batch, p.x_dtype = x_dtype;
   p.out = out, p.out_dtype = out_dtype, p.ldo = ldo, p.out_batch = out_batch;
   p.m = m, p.n = n, p.k = k, p.l = l;
-  int rc = validate_gemv(p, workspace, workspace_bytes, nvfp4_gemv_workspace_bytes(m, k, l));
+  int rc = validate_gemv(p);
   if (rc) return rc;
   const int es = dtype_size(x_dtype);
   p.x_vec = aligned16(x) && ldx * es % 16 == 0 && x_batch * es % 16 == 0;
   DeviceState* d = nullptr;
   if ((rc = get_device(&d))) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, gemv_workspace(x_dtype, p.x_vec, m, n, k, l, d->num_sms)))) return rc;
   if ((rc = encode_operand(&p.map1, b1, n, k, l, kBM))) return rc;
   if (b2 && (rc = encode_operand(&p.map2, b2, n, k, l, kBM))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -1427,10 +1455,9 @@ extern "C" int nvfp4_moe_table(const void* const* b, const void* const* sfb_perm
   return NVFP4_OK;
 }
 
-extern "C" size_t nvfp4_moe_gemv_workspace_bytes(int tokens, int topk, int k) {
-  if (tokens < 1 || topk < 1 || k < 1) return 0;
-  const long long pairs = (long long)tokens * topk;
-  return gemv_space(true, pairs, pairs, k).total;
+extern "C" size_t nvfp4_moe_gemv_workspace_bytes(int x_dtype, int x_aligned, int tokens, int topk, int k) {
+  if (tokens < 1 || topk < 1 || k < 1 || (long long)tokens * topk > kGemvMaxPairs) return 0;
+  return moe_gemv_workspace(x_dtype, x_aligned != 0, tokens * topk, k);
 }
 
 extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_per_pair, const int* expert_ids,
@@ -1440,7 +1467,7 @@ extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_p
   if (tokens < 0 || topk < 1 || num_experts < 1 || n < 1 || k < 1)
     return fail(NVFP4_ERR_INVALID_ARG, "bad sizes (tokens=%d topk=%d experts=%d n=%d k=%d)", tokens, topk, num_experts, n, k);
   if (tokens == 0) return NVFP4_OK;
-  if (!x || !expert_ids || !table1 || !out || !workspace) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
+  if (!x || !expert_ids || !table1 || !out) return fail(NVFP4_ERR_INVALID_ARG, "null pointer argument");
   if ((long long)tokens * topk > kGemvMaxPairs || num_experts > kGemvMaxExperts)
     return fail(NVFP4_ERR_SHAPE, "%d x %d rows (at most %d; the dispatch and the grouped GEMM take more), %d experts (at most %d)",
                 tokens, topk, kGemvMaxPairs, num_experts, kGemvMaxExperts);
@@ -1453,9 +1480,10 @@ extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_p
   p.ids = expert_ids, p.pairs = tokens * topk, p.topk = topk, p.experts = num_experts;
   p.x_per_pair = x_per_pair != 0;
   p.table1 = static_cast<const GemvExpert*>(table1), p.table2 = static_cast<const GemvExpert*>(table2);
-  int rc = validate_gemv(p, workspace, workspace_bytes, nvfp4_moe_gemv_workspace_bytes(tokens, topk, k));
+  int rc = validate_gemv(p);
   if (rc) return rc;
   p.x_vec = aligned16(x) && ldx * dtype_size(x_dtype) % 16 == 0;
+  if ((rc = check_workspace(workspace, workspace_bytes, moe_gemv_workspace(x_dtype, p.x_vec, p.pairs, k)))) return rc;
   DeviceState* d = nullptr;
   if ((rc = get_device(&d))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);

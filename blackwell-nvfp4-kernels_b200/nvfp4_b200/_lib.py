@@ -115,12 +115,12 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     lib.nvfp4_gemv.argtypes = [vp, i32, i64, i64, vp, vp, vp, vp, vp, i32, i64, i64, i32, i32, i32, i32,
                                vp, sz, vp]
     lib.nvfp4_gemv.restype = i32
-    lib.nvfp4_gemv_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.nvfp4_gemv_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
     lib.nvfp4_gemv_workspace_bytes.restype = sz
     lib.nvfp4_moe_gemv.argtypes = [vp, i32, i64, i32, vp, i32, i32, vp, vp, i32, vp, i32, i64, i32, i32,
                                    vp, sz, vp]
     lib.nvfp4_moe_gemv.restype = i32
-    lib.nvfp4_moe_gemv_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.nvfp4_moe_gemv_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     lib.nvfp4_moe_gemv_workspace_bytes.restype = sz
     lib.nvfp4_moe_table.argtypes = [pp, pp, i32, i32, i32, vp]
     lib.nvfp4_moe_table.restype = i32

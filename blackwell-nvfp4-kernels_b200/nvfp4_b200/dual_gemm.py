@@ -78,6 +78,15 @@ def _current_stream_handle(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
+def current_stream_on(index: int):
+    """The raw handle of device ``index``'s current stream if that device is
+    current (the common case, ~0.2 us), else None: the call then goes through
+    :func:`on_device`."""
+    if _get_device is not None and _raw_stream is not None and _get_device() == index:
+        return _raw_stream(index)
+    return None
+
+
 def on_device(device: torch.device, launch):
     """Run launch(stream_handle) with `device` current (the library launches
     on the current device) and its current stream; the device switch is

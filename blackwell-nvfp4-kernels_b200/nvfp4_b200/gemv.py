@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .dual_gemm import check_sf_perm, on_device
+from .dual_gemm import check_sf_perm, current_stream_on, on_device
 from .formats import ceil_div
 
 DTYPES = {torch.float32: _lib.NVFP4_F32, torch.float16: _lib.NVFP4_F16,
@@ -58,38 +58,58 @@ class Weights:
         self.b, self.sfb_perm = b, sfb_perm
         self.n, self.k, self.l, self.device = n, k, l, b.device
         self.ptrs = (b.data_ptr(), sfb_perm.data_ptr())
+        self.space: dict = {}       # workspace bytes by (rows, type and alignment of x)
 
 
 def _rows_last(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _launch(fn, device, args) -> None:
+    """fn(*args, stream) on the device's current stream, with the device current."""
+    st = current_stream_on(device.index)
+    status = fn(*args, st) if st is not None else on_device(device, lambda s: fn(*args, s))
+    if status:
+        _lib.check(status)
+
+
 def _run(x, w, w2, out, out_dtype):
-    if x.dim() not in (2, 3) or x.dtype not in DTYPES:
+    code, dims = DTYPES.get(x.dtype), x.dim()
+    if code is None or dims not in (2, 3):
         raise ValueError("x must be float16, bfloat16 or float32 [M, K] or [L, M, K]")
     if x.device != w.device:
         raise ValueError(f"x is on {x.device}, the weights on {w.device}")
-    batched = x.dim() == 3
-    if x.shape[-1] != w.k or (x.shape[0] if batched else 1) != w.l:
-        raise ValueError(f"x {tuple(x.shape)} does not match weights of K={w.k}, L={w.l}")
-    m = int(x.shape[-2])
+    n, k, l, shape = w.n, w.k, w.l, x.shape
+    if shape[-1] != k or (shape[0] if dims == 3 else 1) != l:
+        raise ValueError(f"x {tuple(shape)} does not match weights of K={k}, L={l}")
+    m = shape[-2]
     x = _rows_last(x)
-    shape = (w.l, m, w.n) if batched else (m, w.n)
+    want = (l, m, n) if dims == 3 else (m, n)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=x.device)
-    elif (tuple(out.shape) != shape or out.dtype not in DTYPES or out.device != x.device
-          or out.dtype != (out_dtype or out.dtype) or (out.stride(-1) != 1 and w.n > 1)
-          or (m > 1 and out.stride(-2) < w.n)
-          or (batched and w.l > 1 and out.stride(0) < (m - 1) * out.stride(1) + w.n)):
-        raise ValueError(f"out must be {shape}, float16, bfloat16 or float32, rows apart, on {x.device}")
+        out = x.new_empty(want, dtype=out_dtype or x.dtype)
+        if out.dtype not in DTYPES:
+            raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
+    elif (tuple(out.shape) != want or out.dtype not in DTYPES or out.device != x.device
+          or out.dtype != (out_dtype or out.dtype) or (out.stride(-1) != 1 and n > 1)
+          or (m > 1 and out.stride(-2) < n)
+          or (dims == 3 and l > 1 and out.stride(0) < (m - 1) * out.stride(1) + n)):
+        raise ValueError(f"out must be {want}, float16, bfloat16 or float32, rows apart, on {x.device}")
+    if m == 0:
+        return out
+    xs, os_, px, es = x.stride(), out.stride(), x.data_ptr(), x.element_size()
+    xb, ob = (xs[0], os_[0]) if dims == 3 else (0, 0)
     lib = _lib.load()
-    b2 = w2.ptrs if w2 is not None else (None, None)
-    size = lib.nvfp4_gemv_workspace_bytes(m, w.k, w.l)
-    space = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _lib.check(on_device(x.device, lambda st: lib.nvfp4_gemv(
-        x.data_ptr(), DTYPES[x.dtype], x.stride(-2), x.stride(0) if batched else 0, *w.ptrs, *b2,
-        out.data_ptr(), DTYPES[out.dtype], max(out.stride(-2), w.n), out.stride(0) if batched else 0,
-        m, w.n, w.k, w.l, space.data_ptr(), size, st)))
+    aligned = not (px | xs[-2] * es | xb * es) & 15
+    size = w.space.get((m, code, aligned))
+    if size is None:
+        with torch.cuda.device(w.device):
+            size = lib.nvfp4_gemv_workspace_bytes(code, aligned, m, n, k, l)
+        w.space[(m, code, aligned)] = size
+    space = x.new_empty(size, dtype=torch.uint8) if size else None
+    _launch(lib.nvfp4_gemv, x.device, (
+        px, code, xs[-2], xb, *w.ptrs, *(w2.ptrs if w2 is not None else (None, None)), out.data_ptr(),
+        DTYPES[out.dtype], os_[-2] if os_[-2] > n else n, ob, m, n, k, l,
+        space.data_ptr() if size else None, size))
     return out
 
 

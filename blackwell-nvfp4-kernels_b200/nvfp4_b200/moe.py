@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .dual_gemm import on_device
-from .gemv import DTYPES, _rows_last
+from .gemv import DTYPES, _launch, _rows_last
 
 
 @dataclass
@@ -153,11 +153,14 @@ class ExpertWeights:
         self.sfb_ptrs = arr(*[s.data_ptr() for _, s in self.w])
         self.device = b0.device
         self._table = None
+        self.space: dict = {}       # workspace bytes by (tokens, topk, type and alignment of x)
 
     def table(self) -> torch.Tensor:
         """The experts' weights as :func:`gemv` finds them in device memory (made by
         the first call that needs it)."""
         if self._table is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call ExpertWeights.table() (or one product) before capturing a CUDA graph")
             lib = _lib.load()
             host = (ctypes.c_char * int(lib.nvfp4_moe_table_bytes(len(self.w))))()
             with torch.cuda.device(self.device):
@@ -217,28 +220,38 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
     ids = expert_ids if expert_ids.dim() == 2 else expert_ids.unsqueeze(1)
     if ids.dim() != 2 or ids.dtype != torch.int32:
         raise ValueError("expert_ids must be int32 [tokens] or [tokens, topk]")
-    if x.dim() != 2 or x.dtype not in DTYPES:
+    code = DTYPES.get(x.dtype)
+    if x.dim() != 2 or code is None:
         raise ValueError("x must be float16, bfloat16 or float32 [tokens or tokens*topk, K]")
     if not (x.device == ids.device == w.device):
         raise ValueError(f"x, expert_ids and the weights must be on one device ({w.device})")
     tokens, topk = ids.shape
-    rows = tokens * topk
-    if x.shape[1] != w.k or x.shape[0] not in (tokens, rows):
-        raise ValueError(f"x {tuple(x.shape)} is neither [{tokens}, {w.k}] nor [{rows}, {w.k}]")
+    rows, n, k = tokens * topk, w.n, w.k
+    if x.shape[1] != k or x.shape[0] not in (tokens, rows):
+        raise ValueError(f"x {tuple(x.shape)} is neither [{tokens}, {k}] nor [{rows}, {k}]")
     x, ids = _rows_last(x), ids.contiguous()
     if out is None:
-        out = torch.empty((rows, w.n), dtype=out_dtype or x.dtype, device=x.device)
-    elif (tuple(out.shape) != (rows, w.n) or out.dtype not in DTYPES or out.device != x.device
-          or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and w.n > 1)
-          or (rows > 1 and out.stride(0) < w.n)):
-        raise ValueError(f"out must be [{rows}, {w.n}], float16, bfloat16 or float32, rows apart, on {x.device}")
+        out = x.new_empty((rows, n), dtype=out_dtype or x.dtype)
+        if out.dtype not in DTYPES:
+            raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
+    elif (tuple(out.shape) != (rows, n) or out.dtype not in DTYPES or out.device != x.device
+          or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and n > 1)
+          or (rows > 1 and out.stride(0) < n)):
+        raise ValueError(f"out must be [{rows}, {n}], float16, bfloat16 or float32, rows apart, on {x.device}")
+    if rows == 0:
+        return out
+    ldx, ldo, px = x.stride(0), out.stride(0), x.data_ptr()
     lib = _lib.load()
-    size = lib.nvfp4_moe_gemv_workspace_bytes(tokens, topk, w.k)
-    space = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _lib.check(on_device(x.device, lambda st: lib.nvfp4_moe_gemv(
-        x.data_ptr(), DTYPES[x.dtype], x.stride(0), int(x.shape[0] == rows and topk > 1), ids.data_ptr(),
-        tokens, topk, w.table().data_ptr(), w2.table().data_ptr() if w2 is not None else None, len(w),
-        out.data_ptr(), DTYPES[out.dtype], max(out.stride(0), w.n), w.n, w.k, space.data_ptr(), size, st)))
+    aligned = not (px | ldx * x.element_size()) & 15
+    size = w.space.get((tokens, topk, code, aligned))
+    if size is None:
+        size = w.space[(tokens, topk, code, aligned)] = lib.nvfp4_moe_gemv_workspace_bytes(code, aligned, tokens,
+                                                                                          topk, k)
+    space = x.new_empty(size, dtype=torch.uint8) if size else None
+    _launch(lib.nvfp4_moe_gemv, x.device, (
+        px, code, ldx, x.shape[0] == rows and topk > 1, ids.data_ptr(), tokens, topk, w.table().data_ptr(),
+        w2.table().data_ptr() if w2 is not None else None, len(w), out.data_ptr(), DTYPES[out.dtype],
+        ldo if ldo > n else n, n, k, space.data_ptr() if size else None, size))
     return out
 
 

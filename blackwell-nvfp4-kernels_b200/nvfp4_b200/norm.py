@@ -16,44 +16,48 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .dual_gemm import on_device
-from .gemv import DTYPES, _rows_last
+from .gemv import DTYPES, _launch, _rows_last
 
 
 def _check(x, weight, residual, residual_out):
     """(x, weight, residual, h): checked, rows with unit stride."""
     if x.dim() != 2 or x.dtype not in DTYPES or not x.is_cuda:
         raise ValueError("x must be a CUDA float16, bfloat16 or float32 tensor [rows, K]")
-    rows, k = x.shape
-    if tuple(weight.shape) != (k,) or weight.dtype not in DTYPES or weight.device != x.device:
-        raise ValueError(f"weight must be float16, bfloat16 or float32 [{k}] on {x.device}")
+    shape, device = x.shape, x.device
+    rows, k = shape
+    if weight.shape != (k,) or weight.dtype not in DTYPES or weight.device != device:
+        raise ValueError(f"weight must be float16, bfloat16 or float32 [{k}] on {device}")
     if k < 1:
         raise ValueError("K must be positive")
-    x, weight = _rows_last(x), weight.contiguous()
+    x = _rows_last(x)
+    if weight.stride(0) != 1:
+        weight = weight.contiguous()
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out without a residual")
         return x, weight, None, None
-    if tuple(residual.shape) != (rows, k) or residual.dtype not in DTYPES or residual.device != x.device:
-        raise ValueError(f"residual must be float16, bfloat16 or float32 [{rows}, {k}] on {x.device}")
+    if residual.shape != shape or residual.dtype not in DTYPES or residual.device != device:
+        raise ValueError(f"residual must be float16, bfloat16 or float32 [{rows}, {k}] on {device}")
     h = residual_out
     if h is None:
-        h = torch.empty((rows, k), dtype=residual.dtype, device=x.device)
-    elif (tuple(h.shape) != (rows, k) or h.dtype != residual.dtype or h.device != x.device
+        h = residual.new_empty(shape)
+    elif (h.shape != shape or h.dtype != residual.dtype or h.device != device
           or (h.stride(1) != 1 and k > 1) or (rows > 1 and h.stride(0) < k)):
-        raise ValueError(f"residual_out must be {residual.dtype} [{rows}, {k}], rows apart, on {x.device}")
+        raise ValueError(f"residual_out must be {residual.dtype} [{rows}, {k}], rows apart, on {device}")
     return x, weight, _rows_last(residual), h
 
 
 def _run(x, weight, residual, h, eps, fmt, y, y_dtype=0, ldy=0, scales=None, group=0, sf_perm=None, sf=None):
-    lib = _lib.load()
     rows, k = x.shape
-    _lib.check(on_device(x.device, lambda st: lib.nvfp4_rms_norm(
-        x.data_ptr(), DTYPES[x.dtype], x.stride(0),
-        *((residual.data_ptr(), DTYPES[residual.dtype], residual.stride(0), h.data_ptr(), max(h.stride(0), k))
-          if residual is not None else (None, 0, 0, None, 0)),
-        weight.data_ptr(), DTYPES[weight.dtype], eps, rows, k, fmt, y, y_dtype, ldy, scales, group, sf_perm, sf,
-        st)))
+    if residual is None:
+        res = (None, 0, 0, None, 0)
+    else:
+        ldh = h.stride(0)
+        res = (residual.data_ptr(), DTYPES[residual.dtype], residual.stride(0), h.data_ptr(),
+               ldh if ldh > k else k)
+    _launch(_lib.load().nvfp4_rms_norm, x.device, (
+        x.data_ptr(), DTYPES[x.dtype], x.stride(0), *res, weight.data_ptr(), DTYPES[weight.dtype], eps, rows, k,
+        fmt, y, y_dtype, ldy, scales, group, sf_perm, sf))
     return x if residual is None else h
 
 
@@ -66,7 +70,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if out is None:
-        out = torch.empty((rows, k), dtype=out_dtype or x.dtype, device=x.device)
+        out = x.new_empty((rows, k), dtype=out_dtype or x.dtype)
+        if out.dtype not in DTYPES:
+            raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
     elif (tuple(out.shape) != (rows, k) or out.dtype not in DTYPES or out.device != x.device
           or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and k > 1)
           or (rows > 1 and out.stride(0) < k)):
@@ -92,8 +98,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
         raise ValueError(f"K={k} must be a multiple of the group ({group})")
     groups = 1 if group is None else k // group
     if out is None:
-        q = torch.empty((rows, k), dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((rows, groups), dtype=torch.float32, device=x.device)
+        q = x.new_empty((rows, k), dtype=torch.float8_e4m3fn)
+        scales = x.new_empty((rows, groups), dtype=torch.float32)
     else:
         q, scales = out
         if (tuple(q.shape) != (rows, k) or tuple(scales.shape) != (rows, groups)
@@ -116,20 +122,20 @@ def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
     if k % 64:
         raise ValueError(f"K={k} must be a multiple of 64")
     rb, ka = -(-rows // 128), k // 64
+    # shapes and strides of quantize.quantize's tensors: views of [1][rows][K/2], [1][rows][K/16] and
+    # [1][rb][ka][32][4][4] bytes
+    views = (((rows, k // 2, 1), (k // 2, 1, rows * (k // 2))), ((rows, k // 16, 1), (k // 16, 1, rows * (k // 16))),
+             ((32, 4, rb, 4, ka, 1), (16, 4, ka * 512, 1, 512, rb * ka * 512)))
     if out is not None:
-        packed = out[0].view(torch.uint8).permute(2, 0, 1)
-        sf = out[1].view(torch.uint8).permute(2, 0, 1)
-        sf_perm = out[2].view(torch.uint8).permute(5, 2, 4, 0, 1, 3)
-        if (tuple(packed.shape) != (1, rows, k // 2) or tuple(sf.shape) != (1, rows, k // 16)
-                or tuple(sf_perm.shape) != (1, rb, ka, 32, 4, 4)
-                or any(t.device != x.device or not t.is_contiguous() for t in (packed, sf, sf_perm))):
-            raise ValueError("out does not match: pass the three tensors an earlier call returned")
+        packed, sf, sf_perm = out
+        for t, (shape, strides), kind in zip(out, views, (torch.float4_e2m1fn_x2,) + (torch.float8_e4m3fn,) * 2):
+            if (tuple(t.shape) != shape or t.dtype != kind or t.device != x.device
+                    or any(a != b for a, b, n in zip(t.stride(), strides, shape) if n > 1)):
+                raise ValueError("out does not match: pass the three tensors an earlier call returned")
     else:
-        packed = torch.empty((1, rows, k // 2), dtype=torch.uint8, device=x.device)
-        sf = torch.empty((1, rows, k // 16), dtype=torch.uint8, device=x.device)
-        sf_perm = torch.empty((1, rb, ka, 32, 4, 4), dtype=torch.uint8, device=x.device)
+        packed = torch.empty_strided(*views[0], dtype=torch.float4_e2m1fn_x2, device=x.device)
+        sf = torch.empty_strided(*views[1], dtype=torch.float8_e4m3fn, device=x.device)
+        sf_perm = torch.empty_strided(*views[2], dtype=torch.float8_e4m3fn, device=x.device)
     h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_NVFP4, packed.data_ptr(), sf_perm=sf_perm.data_ptr(),
              sf=sf.data_ptr())
-    return (packed.permute(1, 2, 0).view(torch.float4_e2m1fn_x2),
-            sf.permute(1, 2, 0).view(torch.float8_e4m3fn),
-            sf_perm.permute(3, 4, 1, 5, 2, 0).view(torch.float8_e4m3fn)), h
+    return (packed, sf, sf_perm), h

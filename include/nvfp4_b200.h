@@ -162,14 +162,15 @@ int nvfp4_moe_combine(const void* c, int c_rows, const int* dst, const float* we
  * Weights and permuted scale atoms as for the GEMMs, K % 64 == 0, any N.
  * An infinity or NaN in x makes that row of out NaN.  m <= 4096; meant for
  * m <= 16, every 16 further rows read the weights again.  `workspace`
- * (nvfp4_gemv_workspace_bytes(), 256-byte aligned) is scratch owned by the call
- * until it completes on `stream`.  No reference counterpart: the reference's GEMMs
+ * (nvfp4_gemv_workspace_bytes() on the same device, may be 0; 256-byte aligned) is
+ * scratch owned by the call until it completes on `stream`; x_aligned: x and its row and
+ * batch strides are multiples of 16 bytes.  No reference counterpart: the reference's GEMMs
  * (nvfp4_dual_gemm/reference.py:27-77) take quantised activations. */
 int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x_batch, const void* b1,
                const void* sf1, const void* b2, const void* sf2, void* out, int out_dtype,
                long long ldo, long long out_batch, int m, int n, int k, int l, void* workspace,
                size_t workspace_bytes, void* stream);
-size_t nvfp4_gemv_workspace_bytes(int m, int k, int l);
+size_t nvfp4_gemv_workspace_bytes(int x_dtype, int x_aligned, int m, int n, int k, int l);
 
 /* The same with each row's own expert: out row r = t*topk + j is x_row . B_eᵀ (or
  * gated, table2 not NULL) with e = expert_ids[r] and x_row = x row t, or x row r when
@@ -185,7 +186,7 @@ int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_per_pair,
                    const int* expert_ids, int tokens, int topk, const void* table1,
                    const void* table2, int num_experts, void* out, int out_dtype, long long ldo,
                    int n, int k, void* workspace, size_t workspace_bytes, void* stream);
-size_t nvfp4_moe_gemv_workspace_bytes(int tokens, int topk, int k);
+size_t nvfp4_moe_gemv_workspace_bytes(int x_dtype, int x_aligned, int tokens, int topk, int k);
 int nvfp4_moe_table(const void* const* b, const void* const* sfb_perm, int num_experts, int n,
                     int k, void* table);
 size_t nvfp4_moe_table_bytes(int num_experts);
