@@ -30,6 +30,7 @@
 
 namespace nvfp4 {
 
+constexpr int kNormAnyType = -1;
 constexpr int kNormPlain = 0, kNormFp8 = 1, kNormNvfp4 = 2;
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxK = kNormMaxThreads * 8 * 4;
@@ -39,7 +40,7 @@ struct NormParams {
   const void *x, *residual, *weight;   // residual may be null
   void* h;                             // [rows][k], the residual's type; null without a residual
   int64_t ldx, ldr, ldh;
-  double eps;
+  double eps, inv_k;                   // inv_k = 1 / k
   int rows, k, x_dtype, r_dtype, w_dtype;
   void* y;                             // plain: [rows][k]; fp8: e4m3 bytes; nvfp4: packed [rows][k/2]
   int64_t ldy;                         // plain only
@@ -53,6 +54,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+// The larger magnitude, with some sign; NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float r;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float largest_of(const float (&v)[8]) {
+  const float a = max_abs_nan(max_abs_nan(v[0], v[1]), max_abs_nan(v[2], v[3]));
+  const float b = max_abs_nan(max_abs_nan(v[4], v[5]), max_abs_nan(v[6], v[7]));
+  return fabsf(max_abs_nan(a, b));
 }
 
 template <bool kVec>
@@ -146,14 +158,30 @@ __device__ __forceinline__ bool norm_fast_scale(float s) {
          (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu;
 }
 
+// v / s (IEEE).  The division itself is kept out of line: it is hardly ever taken.
+__device__ __noinline__ float norm_slow_divide(float v, float s) { return __fdiv_rn(v, s); }
+__device__ __forceinline__ void norm_divide(float (&v)[8], float s, bool fast) {
+  if (fast) {
+    const float rs = __frcp_rn(s);
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = div_by_scale(v[e], s, rs);
+  } else {
+    #pragma unroll 1
+    for (int e = 0; e < 8; ++e) v[e] = norm_slow_divide(v[e], s);
+  }
+}
+
 // One CTA for each row (chunks of 8 elements, chunk c = thread + i * threads,
 // i < NV); kNormNvfp4: CTAs past the rows clear the padding rows of the last
 // block's scale atoms.  kVec: every 8 elements of every tensor are 16-byte aligned
-// and K % 8 == 0.
-template <int NV, int kOut, bool kVec>
-__global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __grid_constant__ NormParams p) {
+// and K % 8 == 0.  kWide: h is fp32.
+//
+// h stays in registers in its own type, half the registers of fp32 for the 16-bit
+// types: several CTAs fit on an SM, whose loads and arithmetic overlap.
+template <int NV, int kOut, bool kVec, int kType>
+__global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ double s_sum[32];
-  __shared__ float s_max[32];
+  __shared__ float s_max[32], s_r;
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
   griddep_wait();
   griddep_launch_dependents();
@@ -170,104 +198,117 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
     }
   }
   const int row = (int)blockIdx.x;
-  float v[NV][8];
-  Raw8 wt[NV];
-  #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (tid + i * (int)blockDim.x) * 8;
-    const Raw8 rx = norm_load8<kVec>(p.x, p.x_dtype, (int64_t)row * p.ldx + col, p.k - col);
-    widen8(rx, p.x_dtype, v[i]);
-    wt[i] = norm_load8<kVec>(p.weight, p.w_dtype, col, p.k - col);
-  }
-  if (p.residual != nullptr) {
+  auto col_of = [&](int i) { return (tid + i * (int)blockDim.x) * 8; };
+  const bool add = p.residual != nullptr;
+  const int x_dtype = kType == kNormAnyType ? p.x_dtype : kType, r_dtype = kType == kNormAnyType ? p.r_dtype : kType;
+  const int w_dtype = kType == kNormAnyType ? p.w_dtype : kType, h_dtype = add ? r_dtype : x_dtype;
+  Raw8 h[NV], wt;
+  double sum = 0.0;
+  {
+    Raw8 rr[NV];
+    #pragma unroll
+    for (int i = 0; i < NV; ++i)
+      h[i] = norm_load8<kVec>(p.x, x_dtype, (int64_t)row * p.ldx + col_of(i), p.k - col_of(i));
+    if (add) {
+      #pragma unroll
+      for (int i = 0; i < NV; ++i)
+        rr[i] = norm_load8<kVec>(p.residual, r_dtype, (int64_t)row * p.ldr + col_of(i), p.k - col_of(i));
+    }
+    if constexpr (NV == 1) wt = norm_load8<kVec>(p.weight, w_dtype, col_of(0), p.k - col_of(0));
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (tid + i * (int)blockDim.x) * 8;
-      const Raw8 rr = norm_load8<kVec>(p.residual, p.r_dtype, (int64_t)row * p.ldr + col, p.k - col);
       float f[8];
-      widen8(rr, p.r_dtype, f);
+      widen8(h[i], x_dtype, f);
+      if (add) {
+        float g[8];
+        widen8(rr[i], r_dtype, g);
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __fadd_rn(f[e], g[e]);
+        h[i] = norm_round(f, r_dtype);
+        norm_store8<kVec>(p.h, r_dtype, (int64_t)row * p.ldh + col_of(i), p.k - col_of(i), h[i]);
+      }
       #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(v[i][e], f[e]);
-      const Raw8 h = norm_round(v[i], p.r_dtype);
-      norm_store8<kVec>(p.h, p.r_dtype, (int64_t)row * p.ldh + col, p.k - col, h);
+      for (int e = 0; e < 8; ++e) {
+        const double d = (double)f[e];
+        sum = fma(d, d, sum);
+      }
     }
   }
-  double sum = 0.0;
-  #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double d = (double)v[i][e];
-      sum = fma(d, d, sum);
-    }
   #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float r;
   if (warps > 1) {
+    // one warp adds up and takes the root: its 50 instructions in every warp would cost
+    // more than the second barrier
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    sum = lane < warps ? s_sum[lane] : 0.0;
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (warp == 0) {
+      sum = lane < warps ? s_sum[lane] : 0.0;
+      #pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_r = (float)rsqrt(fma(sum, p.inv_k, p.eps));
+    }
+    __syncthreads();
+    r = s_r;
+  } else {
+    r = (float)rsqrt(fma(sum, p.inv_k, p.eps));
   }
-  const float r = (float)(1.0 / sqrt(sum / p.k + p.eps));
-  #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  auto values = [&](int i, float (&v)[8]) {               // y of chunk i
     float w[8];
-    widen8(wt[i], p.w_dtype, w);
+    if constexpr (NV > 1) wt = norm_load8<kVec>(p.weight, w_dtype, col_of(i), p.k - col_of(i));
+    widen8(wt, w_dtype, w);
+    widen8(h[i], h_dtype, v);
     #pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], r), w[e]);
-  }
+    for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
+  };
 
   if constexpr (kOut == kNormPlain) {
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (tid + i * (int)blockDim.x) * 8;
-      norm_store8<kVec>(p.y, p.y_dtype, (int64_t)row * p.ldy + col, p.k - col, norm_round(v[i], p.y_dtype));
+      float v[8];
+      values(i, v);
+      norm_store8<kVec>(p.y, p.y_dtype, (int64_t)row * p.ldy + col_of(i), p.k - col_of(i), norm_round(v, p.y_dtype));
     }
   } else if constexpr (kOut == kNormFp8) {
-    float top[NV];
-    #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      // chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then
-      top[i] = 0.f;
-      #pragma unroll
-      for (int e = 0; e < 8; ++e) top[i] = max_nan(top[i], fabsf(v[i][e]));
-    }
+    // chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then
+    float row_top = 0.f;
     if (p.group == 0) {
-      float m = top[0];
       #pragma unroll
-      for (int i = 1; i < NV; ++i) m = max_nan(m, top[i]);
-      #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (warps > 1) {
-        if (lane == 0) s_max[warp] = m;
-        __syncthreads();
-        m = lane < warps ? s_max[lane] : 0.f;
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int i = 0; i < NV; ++i) {
+        float v[8];
+        values(i, v);
+        row_top = max_nan(row_top, largest_of(v));
       }
       #pragma unroll
-      for (int i = 0; i < NV; ++i) top[i] = m;
-    } else {
-      const int lanes = p.group / 8;                      // 4, 8 or 16 neighbouring lanes
-      #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        for (int o = 1; o < lanes; o <<= 1) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      for (int o = 16; o > 0; o >>= 1) row_top = max_nan(row_top, __shfl_xor_sync(0xffffffffu, row_top, o));
+      if (warps > 1) {
+        if (lane == 0) s_max[warp] = row_top;
+        __syncthreads();
+        row_top = lane < warps ? s_max[lane] : 0.f;
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) row_top = max_nan(row_top, __shfl_xor_sync(0xffffffffu, row_top, o));
+      }
     }
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (tid + i * (int)blockDim.x) * 8;
-      const int left = p.k - col;
-      const float s = __fdiv_rn(top[i], 448.f);
+      float v[8];
+      values(i, v);
+      float top = row_top;
+      if (p.group != 0) {
+        top = largest_of(v);
+        for (int o = 1; o < p.group / 8; o <<= 1)         // 4, 8 or 16 neighbouring lanes
+          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      const int col = col_of(i), left = p.k - col;
+      // 448 = 1.75 * 2^8: a mantissa of the exhaustive proof in quantize.cuh
+      const float s = top >= 8.077936e-28f && top <= 3.402823466e38f ? div_by_scale(top, 448.f, 1.f / 448.f)
+                                                                     : norm_slow_divide(top, 448.f);
       uint32_t code[2] = {0u, 0u};
       if (s != 0.f) {
-        const bool fast = norm_fast_scale(s);
-        const float rs = fast ? __frcp_rn(s) : 0.f;
+        norm_divide(v, s, norm_fast_scale(s));
         #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const float q0 = fast ? div_by_scale(v[i][e], s, rs) : __fdiv_rn(v[i][e], s);
-          const float q1 = fast ? div_by_scale(v[i][e + 1], s, rs) : __fdiv_rn(v[i][e + 1], s);
-          const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3);
           code[e / 4] |= two << (8 * (e % 4));
         }
       }
@@ -291,10 +332,10 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
     const int sub = lane & 7;                             // chunk of the 64-column atom
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (tid + i * (int)blockDim.x) * 8;
-      float amax = 0.f;
-      #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(v[i][e]));
+      float v[8];
+      values(i, v);
+      const int col = col_of(i);
+      float amax = largest_of(v);
       amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       const bool finite = amax <= 3.402823466e38f;
       const float a6 = finite ? div_by_scale(amax, 6.0f, 1.0f / 6.0f) : amax;
@@ -302,13 +343,9 @@ __global__ void __launch_bounds__(NV == 4 ? 1024 : 1024) norm_kernel(const __gri
       const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(s8, __NV_E4M3)));
       uint32_t word = 0;
       if (s != 0.f) {
-        const float rs = __frcp_rn(s);
+        norm_divide(v, s, finite);
         #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float q0 = finite ? div_by_scale(v[i][e], s, rs) : __fdiv_rn(v[i][e], s);
-          const float q1 = finite ? div_by_scale(v[i][e + 1], s, rs) : __fdiv_rn(v[i][e + 1], s);
-          word |= e2m1x2(q0, q1) << (4 * e);
-        }
+        for (int e = 0; e < 8; e += 2) word |= e2m1x2(v[e], v[e + 1]) << (4 * e);
       }
       const uint32_t pair = (uint32_t)s8 | (__shfl_down_sync(0xffffffffu, (uint32_t)s8, 2) << 8);
       const uint32_t sf_word = pair | (__shfl_down_sync(0xffffffffu, pair, 4) << 16);   // sub 0

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .gemv import DTYPES, _launch, _rows_last
+from .gemv import DTYPES, _launch, _new, _rows_last
 
 
 def _check(x, weight, residual, residual_out):
@@ -40,7 +40,7 @@ def _check(x, weight, residual, residual_out):
         raise ValueError(f"residual must be float16, bfloat16 or float32 [{rows}, {k}] on {device}")
     h = residual_out
     if h is None:
-        h = residual.new_empty(shape)
+        h = _new((rows, k), residual.dtype, device)
     elif (h.shape != shape or h.dtype != residual.dtype or h.device != device
           or (h.stride(1) != 1 and k > 1) or (rows > 1 and h.stride(0) < k)):
         raise ValueError(f"residual_out must be {residual.dtype} [{rows}, {k}], rows apart, on {device}")
@@ -70,7 +70,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if out is None:
-        out = x.new_empty((rows, k), dtype=out_dtype or x.dtype)
+        out = _new((rows, k), out_dtype or x.dtype, x.device)
         if out.dtype not in DTYPES:
             raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
     elif (tuple(out.shape) != (rows, k) or out.dtype not in DTYPES or out.device != x.device
@@ -98,8 +98,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
         raise ValueError(f"K={k} must be a multiple of the group ({group})")
     groups = 1 if group is None else k // group
     if out is None:
-        q = x.new_empty((rows, k), dtype=torch.float8_e4m3fn)
-        scales = x.new_empty((rows, groups), dtype=torch.float32)
+        q = _new((rows, k), torch.float8_e4m3fn, x.device)
+        scales = _new((rows, groups), torch.float32, x.device)
     else:
         q, scales = out
         if (tuple(q.shape) != (rows, k) or tuple(scales.shape) != (rows, groups)
