@@ -1496,7 +1496,7 @@ extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_p
 namespace nvfp4 {
 namespace {
 
-template <int NV, int kOut, bool kVec, int kType>
+template <int NV, int kThreads, int kOut, bool kVec, int kType>
 int launch_norm_as(const NormParams& p, int threads, cudaStream_t stream) {
   const int pad = kOut == kNormNvfp4 && p.rows % 128 ? (p.k / 64 + kNormPadAtoms - 1) / kNormPadAtoms : 0;
   cudaLaunchConfig_t cfg = {};
@@ -1508,7 +1508,7 @@ int launch_norm_as(const NormParams& p, int threads, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = t_pdl ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm_kernel<NV, kOut, kVec, kType>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm_kernel<NV, kThreads, kOut, kVec, kType>, p);
   if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "norm_kernel launch: %s", cudaGetErrorString(e));
   return check_launch("norm_kernel");
 }
@@ -1518,14 +1518,14 @@ int launch_norm(DeviceState* d, const NormParams& p, cudaStream_t stream) {
   const int chunks = (p.k + 7) / 8;
   // chunks of a thread: one while a row fits (the shortest time for a row), two where there are
   // rows enough for several CTAs on each SM and the row is long (fewer instructions an element):
-  // 1 x 7168 bf16 to fp8 3.0 / 3.6 us with 1 / 2 chunks, 8192 x 7168 111 / 89 us, 4096 x 1024 9.4 / 10.6 us
+  // 1 x 7168 bf16 to fp8 2.9 / 3.5 us with 1 / 2 chunks, 8192 x 7168 111 / 83 us, 4096 x 1024 9.5 / 10.3 us
   int nv = chunks <= kNormMaxThreads ? 1 : chunks <= 2 * kNormMaxThreads ? 2 : 4;
   if (nv == 1 && p.rows >= 2 * d->num_sms && chunks >= 512) nv = 2;
-  if (getenv("NORM_NV")) nv = atoi(getenv("NORM_NV"));
   const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
-  if (nv == 1) return launch_norm_as<1, kOut, kVec, kType>(p, threads, stream);
-  if (nv == 2) return launch_norm_as<2, kOut, kVec, kType>(p, threads, stream);
-  return launch_norm_as<4, kOut, kVec, kType>(p, threads, stream);
+  if (nv == 1) return launch_norm_as<1, 1024, kOut, kVec, kType>(p, threads, stream);
+  if (nv == 2 && threads <= 512) return launch_norm_as<2, 512, kOut, kVec, kType>(p, threads, stream);
+  if (nv == 2) return launch_norm_as<2, 1024, kOut, kVec, kType>(p, threads, stream);
+  return launch_norm_as<4, 1024, kOut, kVec, kType>(p, threads, stream);
 }
 
 template <int kOut>
