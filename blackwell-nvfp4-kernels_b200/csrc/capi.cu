@@ -1207,7 +1207,6 @@ extern "C" int nvfp4_dual_gemm_noalloc(const void* a, const void* b1, const void
 namespace nvfp4 {
 namespace {
 
-
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Device workspace of a call: [groups (experts)][factors][images].
@@ -1231,7 +1230,7 @@ GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
 int gemv_splits(long long tiles, int k_blocks, int num_sms) {
   int best = 1;
   long long least = 0;
-  for (int s = 1; s <= kGemvMaxSplits && s <= k_blocks; s *= 2) {
+  for (int s = 1; s <= kGemvMaxSplits && s <= k_blocks && s <= num_sms; s *= 2) {
     const long long clusters = num_sms / s;
     const long long load = (tiles + clusters - 1) / clusters * ((k_blocks + s - 1) / s + (s > 1 ? 3 : 0));
     if (s == 1 || load < least) best = s, least = load;
@@ -1352,6 +1351,8 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.w_slots &= ~1;
   const int smem = 1024 + p.w_slots * kGemvWBytes + p.x_slots * x_bytes + sums;
   // TMEM: two accumulators (twice where there is room) and the slots' scales
+  // (two CTAs share an SM only under the 112 KB budget: at most 4 weight slots and 8 tokens, 256
+  // columns each, so that neither waits for columns of the other while its cluster waits for it)
   const int n_pad = (p.group_rows * kGemvTerms + 15) / 16 * 16, sf_cols = kGemvSfCols * p.w_slots;
   p.acc_bufs = 4 * n_pad + sf_cols <= 256 ? 2 : 2 * n_pad + sf_cols <= 256 ? 1 : 4 * n_pad + sf_cols <= 512 ? 2 : 1;
   const int cols = p.acc_bufs * 2 * n_pad + sf_cols;
@@ -1367,7 +1368,8 @@ int dtype_size(int t) { return t == kDtF32 ? 4 : 2; }
 bool dtype_ok(int t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
 
 // Sizes, types and alignment that all the products share.
-constexpr int kGemvMaxRows = 4096;   // rows of x in a batch entry
+constexpr int kGemvMaxRows = 4096;       // rows of x in a batch entry
+constexpr int kGemvMaxK = 1 << 20;
 
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (bytes < need || (need > 0 && !workspace))
@@ -1380,8 +1382,11 @@ int check_workspace(const void* workspace, size_t bytes, size_t need) {
 int validate_gemv(const GemvParams& p) {
   if (!dtype_ok(p.x_dtype) || !dtype_ok(p.out_dtype)) return fail(NVFP4_ERR_INVALID_ARG, "bad dtype (x %d, out %d)", p.x_dtype, p.out_dtype);
   if (p.k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", p.k);
-  if ((long long)p.n * p.k * p.l >= (1LL << 41) || (long long)p.m * p.l * p.k >= (1LL << 31))
-    return fail(NVFP4_ERR_SHAPE, "problem too large");
+  if (p.k > kGemvMaxK) return fail(NVFP4_ERR_SHAPE, "K=%d (at most %d)", p.k, kGemvMaxK);
+  // kernels count tiles (row blocks of every 16 rows of x, or of every choice) and x's elements in 32 bits
+  const long long groups = p.pairs ? p.pairs : (long long)p.l * ((p.m + kGemvTokens - 1) / kGemvTokens);
+  if (groups * (p.n / kBM + 1LL) >= (1LL << 30) || (long long)p.m * p.l * p.k >= (1LL << 31))
+    return fail(NVFP4_ERR_SHAPE, "problem too large (m=%d n=%d k=%d l=%d)", p.m, p.n, p.k, p.l);
   if (p.ldx < 0 || p.ldo < p.n) return fail(NVFP4_ERR_INVALID_ARG, "bad row strides (x %lld, out %lld)", (long long)p.ldx, (long long)p.ldo);
   if ((reinterpret_cast<uintptr_t>(p.x) & (dtype_size(p.x_dtype) - 1)) ||
       (reinterpret_cast<uintptr_t>(p.out) & (dtype_size(p.out_dtype) - 1)))

@@ -156,16 +156,17 @@ int nvfp4_moe_combine(const void* c, int c_rows, const int* dst, const float* we
 /* A few tokens times NVFP4 weights: out[l] = x[l] . B1[l]ᵀ, or with b2 / sf2
  * not NULL silu(x[l] . B1[l]ᵀ) * (x[l] . B2[l]ᵀ), for l batch entries.  x [m][k]
  * (rows ldx elements apart, batch entries x_batch) is not quantised; it enters the sums
- * with an error of at most 2^-23 of the largest of its 16 consecutive
- * elements, the sums are fp32, out [m][n] (rows ldo >= n elements apart, batch entries
- * out_batch) is rounded once.  x_dtype and out_dtype are NVFP4_F32, _F16 or _BF16.
- * Weights and permuted scale atoms as for the GEMMs, K % 64 == 0, any N.
- * An infinity or NaN in x makes that row of out NaN.  m <= 4096; meant for
+ * with an error below 2^-22 of the largest of its 16 consecutive elements (or of
+ * 2^-14 of the row's largest, if that is more), the sums are fp32, out [m][n] (rows
+ * ldo >= n elements apart, batch entries out_batch; overlapping neither x nor the
+ * weights) is rounded once.  x_dtype and out_dtype are NVFP4_F32, _F16 or _BF16.
+ * Weights and permuted scale atoms as for the GEMMs, K % 64 == 0, any N.  An infinity or
+ * NaN in x makes that row of out NaN.  m <= 4096, l <= 4096, k <= 2^20; meant for
  * m <= 16, every 16 further rows read the weights again.  `workspace`
  * (nvfp4_gemv_workspace_bytes() on the same device, may be 0; 256-byte aligned) is
  * scratch owned by the call until it completes on `stream`; x_aligned: x and its row and
- * batch strides are multiples of 16 bytes.  No reference counterpart: the reference's GEMMs
- * (nvfp4_dual_gemm/reference.py:27-77) take quantised activations. */
+ * batch strides are multiples of 16 bytes.  No reference counterpart: the reference's
+ * GEMMs (nvfp4_dual_gemm/reference.py:27-77) take quantised activations. */
 int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x_batch, const void* b1,
                const void* sf1, const void* b2, const void* sf2, void* out, int out_dtype,
                long long ldo, long long out_batch, int m, int n, int k, int l, void* workspace,

@@ -1,0 +1,123 @@
+"""CPU: the norm's and the products' entry points reject bad arguments before
+touching a GPU, and their Python sides bad tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from nvfp4_b200 import _lib
+from nvfp4_b200 import build as B
+from nvfp4_b200 import gemv, moe, norm
+
+P, ODD = ctypes.c_void_p(4096), ctypes.c_void_p(4096 + 8)   # never dereferenced
+F32, F16, BF16 = _lib.NVFP4_F32, _lib.NVFP4_F16, _lib.NVFP4_BF16
+INVALID, SHAPE, ALIGNMENT = _lib.NVFP4_ERR_INVALID_ARG, _lib.NVFP4_ERR_SHAPE, _lib.NVFP4_ERR_ALIGNMENT
+
+
+@pytest.fixture(scope="module")
+def lib():
+    B.build()
+    return _lib.load()
+
+
+def _gemv(lib, **k):
+    a = dict(x=P, xt=F16, ldx=256, xb=0, b1=P, s1=P, b2=None, s2=None, out=P, ot=F16, ldo=128, ob=0, m=1, n=128, k=256,
+             l=1, ws=P, size=1 << 30)
+    a.update(k)
+    return lib.nvfp4_gemv(a["x"], a["xt"], a["ldx"], a["xb"], a["b1"], a["s1"], a["b2"], a["s2"], a["out"], a["ot"],
+                          a["ldo"], a["ob"], a["m"], a["n"], a["k"], a["l"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(x=None), INVALID), (dict(b1=None), INVALID), (dict(s1=None), INVALID), (dict(out=None), INVALID),
+    (dict(b2=P), INVALID), (dict(s2=P), INVALID), (dict(m=-1), INVALID), (dict(n=0), INVALID), (dict(k=0), INVALID),
+    (dict(l=0), INVALID), (dict(xt=7), INVALID), (dict(ot=-1), INVALID), (dict(ldo=100), INVALID), (dict(ldx=-1), INVALID),
+    (dict(k=96, ldx=96), SHAPE), (dict(m=5000), SHAPE), (dict(l=5000), SHAPE), (dict(k=1 << 21, ldx=1 << 21), SHAPE),
+    (dict(m=4096, n=1 << 29, ldo=1 << 29), SHAPE), (dict(m=4096, l=4096, k=1 << 20), SHAPE),
+    (dict(b1=ODD), ALIGNMENT), (dict(s1=ODD), ALIGNMENT), (dict(b2=ODD, s2=P), ALIGNMENT),
+    (dict(x=ctypes.c_void_p(4097)), ALIGNMENT), (dict(out=ctypes.c_void_p(4098), ot=F32), ALIGNMENT)])
+def test_gemv_rejects_without_gpu(lib, change, status):
+    assert _gemv(lib, **change) == status
+    assert lib.nvfp4_last_error()
+
+
+def test_gemv_no_rows_and_workspace_sizes(lib):
+    assert _gemv(lib, m=0, x=None) == _lib.NVFP4_OK
+    small, large = (lib.nvfp4_gemv_workspace_bytes(F32, 0, m, 128, 4096, 1) for m in (16, 64))
+    assert 0 < small < large
+    assert lib.nvfp4_gemv_workspace_bytes(F16, 1, 0, 128, 256, 1) == 0
+    assert lib.nvfp4_moe_gemv_workspace_bytes(F16, 1, 4, 8, 1024) == 0          # expanded by the kernel itself
+    assert lib.nvfp4_moe_gemv_workspace_bytes(F16, 0, 4, 8, 1024) > 0
+    assert lib.nvfp4_moe_gemv_workspace_bytes(F16, 1, 5, 8, 1024) > 0
+    assert lib.nvfp4_moe_gemv_workspace_bytes(F16, 1, 1000, 8, 1024) == 0       # refused by the call
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(x=None), INVALID), (dict(ids=None), INVALID), (dict(t1=None), INVALID), (dict(out=None), INVALID),
+    (dict(tokens=-1), INVALID), (dict(topk=0), INVALID), (dict(e=0), INVALID), (dict(n=0), INVALID),
+    (dict(tokens=65, topk=4), SHAPE), (dict(e=1025), SHAPE), (dict(k=100), SHAPE), (dict(xt=3), INVALID),
+    (dict(t1=ctypes.c_void_p(4096 + 16)), ALIGNMENT), (dict(tokens=9, ws=None, size=0), INVALID),
+    (dict(tokens=9, size=64), INVALID), (dict(tokens=9, ws=ODD), ALIGNMENT)])
+def test_moe_gemv_rejects_without_gpu(lib, change, status):
+    a = dict(x=P, xt=F16, ldx=256, per=0, ids=P, tokens=1, topk=4, t1=P, t2=None, e=8, out=P, ot=F16, ldo=128, n=128, k=256,
+             ws=P, size=1 << 30)
+    a.update(change)
+    assert lib.nvfp4_moe_gemv(a["x"], a["xt"], a["ldx"], a["per"], a["ids"], a["tokens"], a["topk"], a["t1"], a["t2"], a["e"],
+                              a["out"], a["ot"], a["ldo"], a["n"], a["k"], a["ws"], a["size"], None) == status
+
+
+def test_moe_table_rejects_without_gpu(lib):
+    one = (ctypes.c_void_p * 1)(4096)
+    odd = (ctypes.c_void_p * 1)(4100)
+    none = (ctypes.c_void_p * 1)(None)
+    buf = (ctypes.c_char * int(lib.nvfp4_moe_table_bytes(1)))()
+    assert lib.nvfp4_moe_table_bytes(0) == 0 and lib.nvfp4_moe_table_bytes(3) == 3 * len(buf)
+    assert lib.nvfp4_moe_table(one, one, 0, 128, 256, buf) == INVALID
+    assert lib.nvfp4_moe_table(one, one, 1, 128, 256, None) == INVALID
+    assert lib.nvfp4_moe_table(none, one, 1, 128, 256, buf) == INVALID
+    assert lib.nvfp4_moe_table(one, odd, 1, 128, 256, buf) == ALIGNMENT
+    assert lib.nvfp4_moe_table(one, one, 1, 128, 100, buf) == SHAPE
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(x=None), INVALID), (dict(w=None), INVALID), (dict(y=None), INVALID), (dict(h=None), INVALID),
+    (dict(rows=-1), INVALID), (dict(k=0), INVALID), (dict(fmt=5), INVALID), (dict(xt=9), INVALID), (dict(eps=-1.0), INVALID),
+    (dict(eps=float("nan")), INVALID), (dict(k=40000, ldh=40000), SHAPE), (dict(fmt=1, scales=None), INVALID),
+    (dict(fmt=1, group=48), SHAPE), (dict(fmt=1, group=128, k=192), SHAPE), (dict(fmt=2, k=100), SHAPE),
+    (dict(fmt=2, sf=None), INVALID), (dict(fmt=2, y=ODD), ALIGNMENT), (dict(ldh=10), INVALID), (dict(fmt=0, ldy=10), INVALID),
+    (dict(x=ctypes.c_void_p(4097)), ALIGNMENT), (dict(fmt=1, scales=ctypes.c_void_p(4098)), ALIGNMENT)])
+def test_rms_norm_rejects_without_gpu(lib, change, status):
+    a = dict(x=P, xt=BF16, ldx=256, r=P, rt=BF16, ldr=256, h=P, ldh=256, w=P, wt=BF16, eps=1e-6, rows=4, k=256, fmt=0, y=P,
+             yt=BF16, ldy=256, scales=P, group=128, sf=P, sfp=None)
+    a.update(change)
+    assert lib.nvfp4_rms_norm(a["x"], a["xt"], a["ldx"], a["r"], a["rt"], a["ldr"], a["h"], a["ldh"], a["w"], a["wt"], a["eps"],
+                              a["rows"], a["k"], a["fmt"], a["y"], a["yt"], a["ldy"], a["scales"], a["group"], a["sf"],
+                              a["sfp"], None) == status
+    assert a["rows"] == 0 or lib.nvfp4_last_error()
+
+
+def test_python_sides_refuse_host_tensors():
+    b, sf = torch.zeros(128, 128, dtype=torch.uint8), torch.zeros(1, 4, 32, 4, 4, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="CUDA"):
+        gemv.Weights(b, sf)
+    with pytest.raises(ValueError, match="CUDA"):
+        norm.rms_norm(torch.zeros(2, 64), torch.zeros(64))
+    with pytest.raises(ValueError):
+        moe.ExpertWeights([(b, sf)])
+    order = moe.pair_order(3, 2, "cpu")
+    assert order.dst.tolist() == list(range(6)) and (order.tokens, order.topk) == (3, 2)
+
+
+def test_digits_of_x_stay_within_their_bound():
+    """The arithmetic of the products' digits on the host: eight balanced base-8 digits in
+    halves are e2m1 values of at most 2 in magnitude and give back x to 2^-23 of the scale."""
+    import numpy as np
+    rng = np.random.default_rng(0)
+    x = np.concatenate([rng.uniform(-1.5, 1.5, 100000), [1.5, -1.5, 0.0, 2.0 ** -24, -(2.0 ** -23)]])   # in units of s
+    units = np.rint(x * 2.0 ** 22).astype(np.int64)
+    fields = units + 0x924924
+    assert (fields >= 0).all() and (fields < 1 << 24).all()
+    digits = np.stack([((fields >> (3 * (7 - j))) & 7) - 4 for j in range(8)])
+    assert digits.min() >= -4 and digits.max() <= 3
+    back = sum(d / 2 * 8.0 ** -j for j, d in enumerate(digits))
+    assert np.abs(back - x).max() <= 2.0 ** -23
