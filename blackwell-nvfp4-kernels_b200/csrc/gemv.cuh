@@ -411,7 +411,6 @@ constexpr int kGemvWBytes = kBM * kBK / 2 + kSfStageBytes;   // a weight slot: 1
 constexpr int kGemvSfCols = 32;          // TMEM columns of a weight slot: its scales and x's
 constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // x slots a power of two
 constexpr int kGemvSelfTokens = 2;       // largest group that gemv_kernel expands itself
-constexpr int kGemvAhead = 2;            // the expansion is at most a tile ahead of the epilogue
 constexpr int kGemvSelfPairs = 32;       // and the most rows of an expert call
 // warps: epilogue 0-3, expansion 0-7 (without it x copies: 4), then weights, two for the MMAs
 constexpr int gemv_threads(bool self) { return 32 * (self ? 11 : 8); }
@@ -480,7 +479,9 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   __shared__ uint32_t s_tmem_base;
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_top[kGemvSelfTokens];             // expansion: largest magnitudes
-  __shared__ float s_back[kGemvAhead][kGemvSelfTokens];   // and 2^-e of the tokens of tile index % kGemvAhead
+  // of the tokens of tile index % 2: 2^-e, and the row of out (experts)
+  __shared__ float s_back[2][kSelf ? kGemvSelfTokens : kGemvTokens];
+  __shared__ int s_row[2][kGemvTokens];
   __shared__ GemvSmallGroups s_small;
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -751,7 +752,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           named_bar_sync(2, 256);
           seen = tc.group;
         }
-        if (tid < tc.rows) s_back[index % kGemvAhead][tid] = exp2_int(-gemv_exponent(s_top[tid]));
+        if (tid < tc.rows) s_back[index % 2][tid] = exp2_int(-gemv_exponent(s_top[tid]));
         __syncwarp();
         for (int i0 = 0; i0 < items && ok; i0 += 32) {
           if (i0 > 0) load_batch(raw, i0);
@@ -788,6 +789,11 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     int acc_buf = 0;
     auto finish = [&](int t, int index) -> bool {
         const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        // before the wait: a load for each token in the loops below is 0.3 us a token
+        if (row < tc.rows) {
+          if constexpr (!kSelf) s_back[index % 2][row] = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + row) * splits + rank);
+          if constexpr (kMoe) s_row[index % 2][row] = kSelf ? s_small.pair[tc.group][row] : __ldcg(&p.groups->pair[tc.before + row]);
+        }
         bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
         if (splits > 1 && t != cluster)
           ok = ok && ctl.wait_cluster(smem_u32(&bar_sums_free), phase ^ 1u, kDevTimeoutPeers);
@@ -805,7 +811,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * tc.rows * kBM) * 4u);
         auto out_at = [&](int tok) -> int64_t {              // where the token's row of this tile starts
           int64_t at;
-          if constexpr (kMoe) at = (int64_t)(kSelf ? s_small.pair[tc.group][tok] : __ldcg(&p.groups->pair[tc.before + tok])) * p.ldo;
+          if constexpr (kMoe) at = (int64_t)s_row[index % 2][tok] * p.ldo;
           else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
           return at + (int64_t)tc.row_block * kBM;
         };
@@ -819,9 +825,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           for (int i = 0; i < 2; ++i) {
             const int tok = t0 + i;
             if (tok >= tc.rows) break;
-            float back;
-            if constexpr (kSelf) back = s_back[index % kGemvAhead][tok];
-            else back = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + tok) * splits + rank);
+            const float back = s_back[index % 2][tok];
             float v[2] = {0.f, 0.f};
             #pragma unroll
             for (int a = 0; a < 2; ++a)
