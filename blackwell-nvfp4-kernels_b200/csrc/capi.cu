@@ -1221,17 +1221,25 @@ GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
   return s;
 }
 
+// Clusters of `splits` CTAs that run at once.  Eight CTAs that need an SM each
+// (more than 8 tokens: see the shared memory below) find neighbouring SMs for about half of the
+// GPU: 16 tokens 2048 x 7168, 16 clusters, 14.9 us, and 9.6 with clusters of 4; 512 x 16384,
+// 4 clusters, 10.0 us and 11.8.
+int gemv_clusters(int splits, int group_rows, int num_sms) {
+  return splits == 8 && group_rows > 8 ? (num_sms + 15) / 16 : num_sms / splits;
+}
+
 // CTAs of a cluster that share a tile's K: the count (a power of two, so that
-// the 128 rows divide) with the fewest K blocks on the busiest CTA, when
-// `tiles` tiles go to one CTA per SM.  The exchange of a tile's sums counts as three
-// K blocks (about 1 us).  Measured, us with 1 / 2 / 4 / 8 CTAs, one token: 512 x 1024 4.7 /
-// 5.0 / 5.0 / 5.0, 2048 x 7168 14.7 / 10.8 / 7.9 / 6.8, 4096 x 14336 26.2 / 17.6 / 12.8 /
-// 11.9, 16384 x 7168 17.0 / 17.7 / 18.0 / 25.7; 16 tokens 7168 x 16384 28.6 / 24.2 / 31.0 / 51.4.
-int gemv_splits(long long tiles, int k_blocks, int num_sms) {
+// the 128 rows divide) with the fewest K blocks on the busiest CTA.  The exchange of a
+// tile's sums counts as three K blocks (about 1 us).  Measured, us with 1 / 2 / 4 / 8 CTAs, one
+// token: 512 x 1024 4.7 / 5.0 / 5.0 / 5.0, 2048 x 7168 14.7 / 10.8 / 7.9 / 6.8, 4096 x 14336 26.2 / 17.6 /
+// 12.8 / 11.9, 16384 x 7168 17.0 / 17.7 / 18.0 / 25.7; 16 tokens 7168 x 16384 28.6 / 24.2 / 31.0 / 51.4
+// (with an epilogue 3 us slower than now).
+int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
   int best = 1;
   long long least = 0;
   for (int s = 1; s <= kGemvMaxSplits && s <= k_blocks && s <= num_sms; s *= 2) {
-    const long long clusters = num_sms / s;
+    const long long clusters = gemv_clusters(s, group_rows, num_sms);
     const long long load = (tiles + clusters - 1) / clusters * ((k_blocks + s - 1) / s + (s > 1 ? 3 : 0));
     if (s == 1 || load < least) best = s, least = load;
   }
@@ -1251,7 +1259,7 @@ bool gemv_expands_itself(int x_dtype, bool x_vec, int pairs) { return x_dtype !=
 int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
   const int k_blocks = (k + kBK - 1) / kBK;
   const long long tiles = (long long)l * ((m + kGemvTokens - 1) / kGemvTokens) * ((n + kBM - 1) / kBM);
-  *splits = gemv_splits(tiles, k_blocks, num_sms);
+  *splits = gemv_splits(tiles, k_blocks, num_sms, m < kGemvTokens ? m : kGemvTokens);
   return (k_blocks + *splits - 1) / *splits;
 }
 
@@ -1305,7 +1313,7 @@ int launch_gemv(DeviceState* d, int slot, const GemvParams& p, int smem, long lo
                         1, stream, p, "gemv_expand_kernel");
     if (rc) return rc;
   }
-  const long long most = d->num_sms / p.splits;
+  const long long most = gemv_clusters(p.splits, p.group_rows, d->num_sms);
   const long long clusters = tiles < most ? tiles : most;
   return launch_chained(kern, dim3((unsigned)(clusters * p.splits), 1, 1), gemv_threads(kSelf), smem, p.splits, stream, p,
                         "gemv_kernel");
@@ -1321,15 +1329,15 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.passes = (p.m + kGemvTokens - 1) / kGemvTokens;
   const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
   const long long tiles = (long long)groups * p.row_blocks;
-  p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms);
-  const int span = (p.k_blocks + p.splits - 1) / p.splits;
-  const bool self = kMoe ? gemv_expands_itself(p.x_dtype, p.x_vec, p.pairs)
-                         : gemv_expands_itself(p.x_dtype, p.x_vec, p.m, span);
-  p.room = self ? kGemvSelfTokens : kGemvTokens;
+  p.room = kGemvTokens;
+  bool self = kMoe && gemv_expands_itself(p.x_dtype, p.x_vec, p.pairs);
   // experts: twice the average of an expert's rows, so that the x slots are not sized for what hardly ever comes
-  if (kMoe && !self)
+  if (self) p.room = kGemvSelfTokens;
+  else if (kMoe)
     while (p.room > 4 && (long long)p.room * p.experts >= 4LL * p.pairs) p.room /= 2;
   p.group_rows = rows < p.room ? rows : p.room;
+  p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms, p.group_rows);
+  if (!kMoe) self = gemv_expands_itself(p.x_dtype, p.x_vec, p.m, (p.k_blocks + p.splits - 1) / p.splits);
   const GemvSpace sp = gemv_space(kMoe, kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   p.groups = reinterpret_cast<GemvGroups*>(ws);

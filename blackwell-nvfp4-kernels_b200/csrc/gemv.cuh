@@ -430,6 +430,15 @@ __device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uin
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// Accumulator columns of two or four tokens.
+__device__ __forceinline__ void tmem_ld_terms(uint32_t taddr, uint32_t (&d)[16]) { tmem_ld_32x32b_x16(taddr, d); }
+__device__ __forceinline__ void tmem_ld_terms(uint32_t taddr, uint32_t (&d)[32]) { tmem_ld_32x32b_x32(taddr, d); }
+template <int N>
+__device__ __forceinline__ void tmem_terms_ready(uint32_t (&d)[N]) {
+  #pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(d[i]));
+}
+
 // What a cluster works on: tile t of the call.
 struct GemvTile { int group, row_block, batch, rows, before, expert; };
 
@@ -815,14 +824,17 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
           return at + (int64_t)tc.row_block * kBM;
         };
-        for (int t0 = 0; t0 < tc.rows; t0 += 2) {
-          uint32_t d[2][16];
-          tmem_ld_32x32b_x16(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
-          if (both) tmem_ld_32x32b_x16(acc + n_pad + t0 * kGemvTerms, d[1]);
+        // several tokens a step, which waits once for its loads; the columns behind the last token's
+        // are other accumulators' or scales, and not used
+        constexpr int kStep = kSelf ? 2 : 4;
+        for (int t0 = 0; t0 < tc.rows; t0 += kStep) {
+          uint32_t d[2][kStep * kGemvTerms];
+          tmem_ld_terms(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
+          if (both) tmem_ld_terms(acc + n_pad + t0 * kGemvTerms, d[1]);
           tmem_ld_wait();
-          tmem_regs_ready16(d[0]), tmem_regs_ready16(d[1]);
+          tmem_terms_ready(d[0]), tmem_terms_ready(d[1]);
           #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kStep; ++i) {
             const int tok = t0 + i;
             if (tok >= tc.rows) break;
             const float back = s_back[index % 2][tok];
@@ -858,9 +870,15 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
             float v[kMats];
             #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
-              v[mat] = 0.f;
-              for (int s = 0; s < splits; ++s)
-                v[mat] += __uint_as_float(lds_u32(sums_base + (uint32_t)(((s * kMats + mat) * tc.rows + tok) * own_rows + r) * 4u));
+              float part[kGemvMaxSplits];                  // all loads before the first sum
+              #pragma unroll
+              for (int s = 0; s < kGemvMaxSplits; ++s)
+                if (s < splits)
+                  part[s] = __uint_as_float(lds_u32(sums_base + (uint32_t)(((s * kMats + mat) * tc.rows + tok) * own_rows + r) * 4u));
+              v[mat] = part[0];
+              #pragma unroll
+              for (int s = 1; s < kGemvMaxSplits; ++s)
+                if (s < splits) v[mat] += part[s];
             }
             const int at = rank * own_rows + r;
             if (tc.row_block * kBM + at < p.n)
