@@ -1589,7 +1589,8 @@ extern "C" int nvfp4_rms_norm(const void* x, int x_dtype, long long ldx, const v
   p.x = x, p.residual = residual, p.weight = weight, p.h = residual ? h : nullptr;
   p.ldx = ldx, p.ldr = ldr, p.ldh = ldh, p.eps = eps, p.inv_k = 1.0 / k, p.rows = rows, p.k = k;
   p.x_dtype = x_dtype, p.r_dtype = r_dtype, p.w_dtype = w_dtype;
-  p.y = y, p.ldy = ldy, p.y_dtype = y_dtype, p.scales = scales, p.group = group;
+  p.y = y, p.ldy = ldy, p.y_dtype = y_dtype, p.scales = scales;
+  p.group_bits = group == 32 ? 5 : group == 64 ? 6 : 7;
   p.sf_perm = static_cast<uint8_t*>(sf_perm), p.sf_plain = static_cast<uint8_t*>(sf_plain);
   auto lines = [](const void* q, int dtype, long long ld) { return aligned16(q) && ld * dtype_size(dtype) % 16 == 0; };
   const bool vec = k % 8 == 0 && lines(x, x_dtype, ldx) && lines(weight, w_dtype, 0) &&
@@ -1597,6 +1598,7 @@ extern "C" int nvfp4_rms_norm(const void* x, int x_dtype, long long ldx, const v
                    (format == kNormPlain ? lines(y, y_dtype, ldy) : (reinterpret_cast<uintptr_t>(y) & 7u) == 0);
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (format == kNormPlain) return launch_norm<kNormPlain>(d, p, vec, stream);
+  if (format == kNormFp8 && group == 0) return launch_norm<kNormFp8Row>(d, p, vec, stream);
   if (format == kNormFp8) return launch_norm<kNormFp8>(d, p, vec, stream);
   return launch_norm<kNormNvfp4>(d, p, vec, stream);
 }

@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cstdint>
+#include <type_traits>
 #include "gemv.cuh"
 #include "ptx.cuh"
 #include "quantize.cuh"
@@ -32,6 +33,7 @@ namespace nvfp4 {
 
 constexpr int kNormAnyType = -1;
 constexpr int kNormPlain = 0, kNormFp8 = 1, kNormNvfp4 = 2;
+constexpr int kNormFp8Row = 3;         // the kernel's fp8 with one scale for the row
 constexpr int kNormMaxThreads = 1024;
 constexpr int kNormMaxK = kNormMaxThreads * 8 * 4;
 constexpr int kNormPadAtoms = 8;       // scale atoms whose padding rows one CTA clears
@@ -46,7 +48,7 @@ struct NormParams {
   int64_t ldy;                         // plain only
   int y_dtype;                         // plain only
   float* scales;                       // fp8: [rows][k / group]
-  int group;                           // fp8: 32, 64 or 128 columns, 0 for the row
+  int group_bits;                      // fp8: 5, 6 or 7 for groups of 32, 64 or 128 columns
   uint8_t *sf_perm, *sf_plain;         // nvfp4
 };
 
@@ -123,6 +125,23 @@ __device__ __forceinline__ Raw8 norm_round(float (&f)[8], int dtype) {
   return r;
 }
 
+// Sums of fp16 or bf16 elements, rounded once: what the fp32 sum rounds to as
+// well, since fp32 has two digits more than twice theirs (Figueroa's condition).
+template <int kType>
+__device__ __forceinline__ Raw8 norm_add16(const Raw8& a, const Raw8& b) {
+  using T2 = std::conditional_t<kType == kDtBF16, __nv_bfloat162, __half2>;
+  uint32_t x[4] = {a.a.x, a.a.y, a.a.z, a.a.w};
+  const uint32_t y[4] = {b.a.x, b.a.y, b.a.z, b.a.w};
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T2 t = __hadd2_rn(*reinterpret_cast<const T2*>(&x[i]), *reinterpret_cast<const T2*>(&y[i]));
+    x[i] = *reinterpret_cast<const uint32_t*>(&t);
+  }
+  Raw8 r;
+  r.a = make_uint4(x[0], x[1], x[2], x[3]), r.b = make_uint4(0, 0, 0, 0);
+  return r;
+}
+
 template <bool kVec>
 __device__ __forceinline__ void norm_store8(void* base, int dtype, int64_t at, int left, const Raw8& r) {
   if (left <= 0) return;
@@ -149,25 +168,51 @@ __device__ __forceinline__ void norm_store8(void* base, int dtype, int64_t at, i
   }
 }
 
-// RN(y / s) for a whole group: by the two fused multiply-adds of
-// quantize.cuh's div_by_scale where Markstein's theorem holds (r = RN(1 / s),
-// s's mantissa not all ones, nothing near under- or overflow), else by the
-// division itself.
-__device__ __forceinline__ bool norm_fast_scale(float s) {
-  return s >= 8.077936e-28f /* 2^-90 */ && s <= 1.329228e36f /* 2^120 */ &&
-         (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu;
+// Two fp32 operations in one instruction (each rounded as by itself).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2_down(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
-// v / s (IEEE).  The division itself is kept out of line: it is hardly ever taken.
-__device__ __noinline__ float norm_slow_divide(float v, float s) { return __fdiv_rn(v, s); }
+// v / s (IEEE): by the two fused multiply-adds of quantize.cuh's div_by_scale
+// where Markstein's theorem holds (r = RN(1 / s), s's mantissa not all ones, nothing
+// near under- or overflow: `fast`), else by the division itself.
 __device__ __forceinline__ void norm_divide(float (&v)[8], float s, bool fast) {
   if (fast) {
     const float rs = __frcp_rn(s);
+    const uint64_t s2 = pack2(-s, -s), r2 = pack2(rs, rs);
     #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = div_by_scale(v[e], s, rs);
+    for (int e = 0; e < 8; e += 2) {
+      const uint64_t x = pack2(v[e], v[e + 1]), q = mul2(x, r2);
+      unpack2(fma2(fma2_down(q, s2, x), r2, q), v[e], v[e + 1]);
+    }
   } else {
+    // hardly ever taken: one division in a loop that turns the values round (indexed by the
+    // loop they would lie in local memory, also for the branch above)
     #pragma unroll 1
-    for (int e = 0; e < 8; ++e) v[e] = norm_slow_divide(v[e], s);
+    for (int i = 0; i < 8; ++i) {
+      const float q = __fdiv_rn(v[0], s);
+      #pragma unroll
+      for (int e = 0; e < 7; ++e) v[e] = v[e + 1];
+      v[7] = q;
+    }
   }
 }
 
@@ -220,8 +265,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float f[8];
+      if (kType != kNormAnyType && add) h[i] = norm_add16<kType>(h[i], rr[i]);
       widen8(h[i], x_dtype, f);
-      if (add) {
+      if (kType != kNormAnyType && add) {
+        norm_store8<kVec>(p.h, r_dtype, (int64_t)row * p.ldh + col_of(i), p.k - col_of(i), h[i]);
+      } else if (add) {
         float g[8];
         widen8(rr[i], r_dtype, g);
         #pragma unroll
@@ -261,7 +309,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
     widen8(wt, w_dtype, w);
     widen8(h[i], h_dtype, v);
     #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
+    for (int e = 0; e < 8; e += 2)
+      unpack2(mul2(mul2(pack2(v[e], v[e + 1]), pack2(r, r)), pack2(w[e], w[e + 1])), v[e], v[e + 1]);
   };
 
   if constexpr (kOut == kNormPlain) {
@@ -271,10 +320,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
       values(i, v);
       norm_store8<kVec>(p.y, p.y_dtype, (int64_t)row * p.ldy + col_of(i), p.k - col_of(i), norm_round(v, p.y_dtype));
     }
-  } else if constexpr (kOut == kNormFp8) {
+  } else if constexpr (kOut == kNormFp8 || kOut == kNormFp8Row) {
     // chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then
     float row_top = 0.f;
-    if (p.group == 0) {
+    if constexpr (kOut == kNormFp8Row) {
       #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float v[8];
@@ -296,18 +345,22 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
       float v[8];
       values(i, v);
       float top = row_top;
-      if (p.group != 0) {
+      if constexpr (kOut == kNormFp8) {
         top = largest_of(v);
-        for (int o = 1; o < p.group / 8; o <<= 1)         // 4, 8 or 16 neighbouring lanes
-          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        #pragma unroll
+        for (int o = 1; o < 16; o <<= 1)                  // 4, 8 or 16 neighbouring lanes
+          if (8 * o < 1 << p.group_bits) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
       const int col = col_of(i), left = p.k - col;
-      // 448 = 1.75 * 2^8: a mantissa of the exhaustive proof in quantize.cuh
-      const float s = top >= 8.077936e-28f && top <= 3.402823466e38f ? div_by_scale(top, 448.f, 1.f / 448.f)
-                                                                     : norm_slow_divide(top, 448.f);
+      // 448 = 1.75 * 2^8: a mantissa of the exhaustive proof in quantize.cuh; y and s between
+      // 2^-90 and 2^120 where it matters
+      float s = div_by_scale(top, 448.f, 1.f / 448.f);
+      const bool fast = top >= 3.308722e-24f /* 2^-78 */ && top <= 8.507059e37f /* 2^126 */ &&
+                        (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu;
+      if (!fast) s = __fdiv_rn(top, 448.f);
       uint32_t code[2] = {0u, 0u};
       if (s != 0.f) {
-        norm_divide(v, s, norm_fast_scale(s));
+        norm_divide(v, s, fast);
         #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3);
@@ -323,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
           for (int e = 0; e < 8; ++e)
             if (e < left) q[e] = (uint8_t)(code[e / 4] >> (8 * (e % 4)));
         }
-        if (p.group == 0) {
+        if constexpr (kOut == kNormFp8Row) {
           if (tid == 0 && i == 0) p.scales[row] = s;
-        } else if (col % p.group == 0) {
-          p.scales[(int64_t)row * (p.k / p.group) + col / p.group] = s;
+        } else if ((col & ((1 << p.group_bits) - 1)) == 0) {
+          p.scales[(int64_t)row * (p.k >> p.group_bits) + (col >> p.group_bits)] = s;
         }
       }
     }
