@@ -1530,10 +1530,11 @@ template <int kOut, bool kVec, int kType>
 int launch_norm(DeviceState* d, const NormParams& p, cudaStream_t stream) {
   const int chunks = (p.k + 7) / 8;
   // chunks of a thread: one while a row fits (the shortest time for a row), two where there are
-  // rows enough for several CTAs on each SM and the row is long (fewer instructions an element):
-  // 1 x 7168 bf16 to fp8 2.9 / 3.5 us with 1 / 2 chunks, 8192 x 7168 111 / 83 us, 4096 x 1024 9.5 / 10.3 us
+  // rows enough for several CTAs on each SM and one chunk would make CTAs of more than 512
+  // threads, which leave SMs half empty.  With 1 / 2 chunks, us: 8192 x 7168 bf16 to fp8 84.9 / 67.6;
+  // 777 x 4096 fp16 7.1 / 7.7; 2048 x 4096 to NVFP4 13.4 / 13.6; 4096 x 1024 7.5 / 8.8
   int nv = chunks <= kNormMaxThreads ? 1 : chunks <= 2 * kNormMaxThreads ? 2 : 4;
-  if (nv == 1 && p.rows >= 2 * d->num_sms && chunks >= 512) nv = 2;
+  if (nv == 1 && p.rows >= 2 * d->num_sms && chunks > 512) nv = 2;
   const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
   if (nv == 1) return launch_norm_as<1, 1024, kOut, kVec, kType>(p, threads, stream);
   if (nv == 2 && threads <= 512) return launch_norm_as<2, 512, kOut, kVec, kType>(p, threads, stream);
