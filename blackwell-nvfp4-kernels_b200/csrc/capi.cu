@@ -1309,7 +1309,7 @@ int launch_gemv(DeviceState* d, int slot, const GemvParams& p, int smem, long lo
   if constexpr (!kSelf) {
     const int chunks = ((p.k_blocks + p.splits - 1) / p.splits + kExpandBlocks - 1) / kExpandBlocks;
     const int rows = kMoe ? p.pairs : p.l * p.m;
-    rc = launch_chained(gemv_expand_kernel<kMoe>, dim3((unsigned)rows, (unsigned)(chunks * p.splits), 1), kExpandThreads, 0,
+    rc = launch_chained(gemv_expand_kernel<kMoe>, dim3((unsigned)rows, (unsigned)chunks, (unsigned)p.splits), kExpandThreads, 0,
                         1, stream, p, "gemv_expand_kernel");
     if (rc) return rc;
   }
@@ -1337,6 +1337,7 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
     while (p.room > 4 && (long long)p.room * p.experts >= 4LL * p.pairs) p.room /= 2;
   p.group_rows = rows < p.room ? rows : p.room;
   p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms, p.group_rows);
+  p.split_bits = p.splits == 8 ? 3 : p.splits / 2;
   if (!kMoe) self = gemv_expands_itself(p.x_dtype, p.x_vec, p.m, (p.k_blocks + p.splits - 1) / p.splits);
   const GemvSpace sp = gemv_space(kMoe, kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);

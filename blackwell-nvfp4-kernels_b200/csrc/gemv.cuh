@@ -79,7 +79,7 @@ struct GemvParams {
   int x_vec;                             // every 8 elements of x are 16-byte aligned
   int k_blocks, row_blocks;              // 256-deep K blocks, 128-row blocks
   int passes;                            // groups of 16 tokens of a batch entry
-  int splits;                            // CTAs of a cluster, each with a part of K
+  int splits, split_bits;                // CTAs of a cluster, each with a part of K; splits = 1 << split_bits
   int room, group_rows;                  // tokens that a group can have, and the largest has
   int w_slots, x_slots, acc_bufs;        // shared-memory ring slots, accumulators
   // expansion
@@ -326,7 +326,7 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
     if (group_of[i] >= 0) out.pair[out.before[group_of[i]] + place_of[i]] = i;
 }
 
-// grid: (row of x, chunk of 8 K blocks of a split).  A CTA takes the largest magnitude
+// grid: (row of x, chunk of 8 K blocks, split).  A CTA takes the largest magnitude
 // of its row in the whole split (every CTA of the split reads it: a few KB from L2),
 // then each warp expands one K block.
 template <bool kMoe>
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
   if constexpr (kMoe) {
     if (warp == 0) gemv_group_pairs(p, s_groups, s_seen, s_open, s_group_of, s_place_of);
     __syncthreads();
-    if (r == 0 && blockIdx.y == 0) {
+    if (r == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
       if (tid == 0) p.groups->count = s_groups.count;
       for (int i = tid; i < p.pairs; i += kExpandThreads) {
         p.groups->expert[i] = s_groups.expert[i], p.groups->rows[i] = s_groups.rows[i];
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
     }
     group = s_group_of[r], place = s_place_of[r];
     if (group < 0) {                                      // not an expert: a row of zeros
-      for (int c = (int)blockIdx.y * kExpandThreads + tid; c < p.n; c += (int)gridDim.y * kExpandThreads)
+      for (int c = (int)(blockIdx.z * gridDim.y + blockIdx.y) * kExpandThreads + tid; c < p.n; c += (int)(gridDim.y * gridDim.z) * kExpandThreads)
         store_out(p.out, p.out_dtype, (int64_t)r * p.ldo + c, 0.f);
       return;
     }
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
     rows_all = groups_all = p.pairs;
     src = (int64_t)(p.x_per_pair ? r : r / p.topk) * p.ldx;
   } else {
-    const int batch = r / p.m, row = r % p.m, pass = row / kGemvTokens;
+    const int batch = p.l == 1 ? 0 : r / p.m, row = r - batch * p.m, pass = row / kGemvTokens;
     place = row % kGemvTokens;
     group = batch * p.passes + pass;
     rows = min(kGemvTokens, p.m - pass * kGemvTokens);
@@ -369,9 +369,8 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
     rows_all = p.l * p.m, groups_all = p.l * p.passes;
     src = (int64_t)batch * p.x_batch + (int64_t)row * p.ldx;
   }
-  const int chunks = (int)gridDim.y / p.splits;
-  const int split = (int)blockIdx.y / chunks, chunk = (int)blockIdx.y % chunks;
-  const int kb0 = p.k_blocks * split / p.splits, kb1 = p.k_blocks * (split + 1) / p.splits;
+  const int split = (int)blockIdx.z, chunk = (int)blockIdx.y;
+  const int kb0 = (p.k_blocks * split) >> p.split_bits, kb1 = (p.k_blocks * (split + 1)) >> p.split_bits;
   if (kb0 + chunk * kExpandBlocks >= kb1) return;
 
   // this thread's elements, and the largest of the split
@@ -408,6 +407,8 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
 // Products
 // ---------------------------------------------------------------------------
 constexpr int kGemvWBytes = kBM * kBK / 2 + kSfStageBytes;   // a weight slot: 128 rows x 256, scale atoms
+constexpr int kBMBits = 7;
+static_assert(1 << kBMBits == kBM, "rows of a block");
 constexpr int kGemvSfCols = 32;          // TMEM columns of a weight slot: its scales and x's
 constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // x slots a power of two
 constexpr int kGemvSelfTokens = 2;       // largest group that gemv_kernel expands itself
@@ -446,14 +447,14 @@ struct GemvTile { int group, row_block, batch, rows, before, expert; };
 struct GemvSmallGroups {
   int count;
   int expert[kGemvSelfPairs], rows[kGemvSelfPairs];
-  int pair[kGemvSelfPairs][kGemvSelfTokens];
+  int pair[kGemvSelfPairs][kGemvSelfTokens], x_row[kGemvSelfPairs][kGemvSelfTokens];
 };
 
 template <bool kMoe, bool kSelf>
 __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSmallGroups& small, int t) {
   GemvTile r;
   if constexpr (kMoe) {
-    r.group = t / p.row_blocks, r.row_block = t % p.row_blocks, r.batch = 0;
+    r.group = t / p.row_blocks, r.row_block = t - r.group * p.row_blocks, r.batch = 0;
     if constexpr (kSelf) {
       r.expert = small.expert[r.group], r.rows = small.rows[r.group], r.before = 0;
     } else {
@@ -461,9 +462,10 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSma
       r.rows = __ldcg(&p.groups->rows[r.group]), r.before = __ldcg(&p.groups->before[r.group]);
     }
   } else {
-    // groups of the same weights next to one another: they share them in L2
-    const int pass = t % p.passes, rest = t / p.passes;
-    r.row_block = rest % p.row_blocks, r.batch = rest / p.row_blocks;
+    // groups of the same weights next to one another: they share them in L2 (the branches spare
+    // two divisions, about 0.1 us, where they are not needed)
+    const int rest = p.passes == 1 ? t : t / p.passes, pass = t - rest * p.passes;
+    r.batch = p.l == 1 ? 0 : rest / p.row_blocks, r.row_block = rest - r.batch * p.row_blocks;
     r.group = r.batch * p.passes + pass;
     r.rows = min(kGemvTokens, p.m - pass * kGemvTokens), r.before = r.batch * p.m + pass * kGemvTokens;
     r.expert = 0;
@@ -497,8 +499,8 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   const int warp = (int)threadIdx.x >> 5, lane = (int)(threadIdx.x & 31u);
   const int splits = p.splits;
   const int rank = splits > 1 ? (int)cluster_ctarank() : 0;
-  const int cluster = (int)blockIdx.x / splits, clusters = (int)gridDim.x / splits;
-  const int kb0 = p.k_blocks * rank / splits, kb1 = p.k_blocks * (rank + 1) / splits;
+  const int cluster = (int)blockIdx.x >> p.split_bits, clusters = (int)gridDim.x >> p.split_bits;
+  const int kb0 = (p.k_blocks * rank) >> p.split_bits, kb1 = (p.k_blocks * (rank + 1)) >> p.split_bits;
   // shared memory: weight slots, x slots, the cluster's sums
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;   // a multiple of 1024
   // odd numbers of tokens: 8 columns more, whose digits are whatever lies behind; they are not used
@@ -528,20 +530,23 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   if (warp == kMmaWarp) tmem_alloc<kTmemCols>(smem_u32(&s_tmem_base));
   if constexpr (kMoe) griddep_wait();                     // the experts' ids, or the groups from the expansion
   if constexpr (kMoe && kSelf) {
-    // rows of one expert in ascending order, p.room at a time
+    // rows of one expert in ascending order, kGemvSelfTokens at a time
     if (warp == 0) {
       const uint32_t lt = (1u << lane) - 1u;
       const int id = lane < p.pairs ? __ldg(p.ids + lane) : -1;
       const bool valid = (unsigned)id < (unsigned)p.experts;
       const uint32_t same = __match_any_sync(0xffffffffu, valid ? id : -1);
       const int at = __popc(same & lt);
-      const bool first = valid && at % p.room == 0;
+      const bool first = valid && at % kGemvSelfTokens == 0;
       const uint32_t firsts = __ballot_sync(0xffffffffu, first);
       const uint32_t mine = firsts & same & (lt | (1u << lane));
       const int from = valid ? 31 - __clz(mine) : lane;
       const int grp = __shfl_sync(0xffffffffu, __popc(firsts & lt), from);
-      if (valid) s_small.pair[grp][at % p.room] = lane;
-      if (first) s_small.expert[grp] = id, s_small.rows[grp] = min(p.room, __popc(same) - at);
+      if (valid) {
+        s_small.pair[grp][at % kGemvSelfTokens] = lane;
+        s_small.x_row[grp][at % kGemvSelfTokens] = p.x_per_pair ? lane : lane / p.topk;
+      }
+      if (first) s_small.expert[grp] = id, s_small.rows[grp] = min(kGemvSelfTokens, __popc(same) - at);
       if (lane == 0) s_small.count = __popc(firsts);
     }
   }
@@ -700,7 +705,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     // ------------------------------------------------------------ workers: expansion, epilogue
     griddep_wait();                                       // x or its expansion; and nothing is written before
     const int row = warp * 32 + lane;
-    const int own_rows = kBM / splits, owner = row / own_rows;   // the CTA that finishes this thread's row
+    const int own_bits = kBMBits - p.split_bits, own_rows = 1 << own_bits, owner = row >> own_bits;   // the CTA that finishes this thread's row
     if constexpr (kMoe && kSelf) {                        // rows without an expert are zero
       for (int i = (int)blockIdx.x; i < p.pairs; i += (int)gridDim.x)
         if ((unsigned)__ldg(p.ids + i) >= (unsigned)p.experts)
@@ -718,20 +723,19 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
       if constexpr (kSelf) {                              // x in 16 bits, 16-byte aligned
         const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
         auto x_at = [&](int tok) -> int64_t {
-          if constexpr (kMoe) {
-            const int pr = s_small.pair[tc.group][tok];
-            return (int64_t)(p.x_per_pair ? pr : pr / p.topk) * p.ldx;
-          }
+          if constexpr (kMoe) return (int64_t)s_small.x_row[tc.group][tok] * p.ldx;
           return (int64_t)tc.batch * p.x_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldx;
         };
-        const int items = span * tc.rows, done = index * span;
+        static_assert(kGemvSelfTokens == 2, "token of an item: its last bit");
+        const int two = tc.rows - 1;                        // tokens of the group: 1 or 2
+        const int items = span << two, done = index * span;
         // the elements of four rounds' items at a time
         auto load_batch = [&](uint4 (&r)[4], int i0) {
           #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 8 * u + me, k0 = (kb0 + i / tc.rows) * kBK + lane * 8;
+            const int i = i0 + 8 * u + me, k0 = (kb0 + (i >> two)) * kBK + lane * 8;
             r[u] = make_uint4(0, 0, 0, 0);
-            if (i < items && k0 < p.k) r[u] = ldg_v4(static_cast<const uint16_t*>(p.x) + x_at(i % tc.rows) + k0);
+            if (i < items && k0 < p.k) r[u] = ldg_v4(static_cast<const uint16_t*>(p.x) + x_at(i & two) + k0);
           }
         };
         uint4 raw[4];
@@ -749,7 +753,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
               const int i = i0 + 8 * u + me;
               if (i >= items) break;
               const uint32_t top = __reduce_max_sync(0xffffffffu, largest8(Raw8{r[u], {}}, p.x_dtype));
-              if (lane == 0) atomicMax(&s_top[i % tc.rows], top);
+              if (lane == 0) atomicMax(&s_top[i & two], top);
             }
           };
           take(raw, 0);
@@ -768,8 +772,8 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           #pragma unroll
           for (int u = 0; u < 4; ++u) {
             if (i0 + 8 * u >= items || !ok) break;
-            const int i = i0 + 8 * u + me, tok = i % tc.rows;
-            const int c = done + i / tc.rows, slot = c & slot_mask;
+            const int i = i0 + 8 * u + me, tok = i & two;
+            const int c = done + (i >> two), slot = c & slot_mask;
             bool free = true;
             if (i < items) {                              // the same for the whole warp
               free = ctl.wait(smem_u32(&bar_x_free[slot]), (uint32_t)((c >> slot_bits) & 1) ^ 1u, kDevTimeoutStageFree);
@@ -813,7 +817,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
         const bool both = kDual || kb1 - kb0 > 1;
         const int only = index * (kb1 - kb0) & 1;
         // sums of a sender in an owner's shared memory: [sender][matrix][token][row of the owner]
-        const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + row % own_rows) * 4u;
+        const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + (row & (own_rows - 1))) * 4u;
         const uint32_t remote = splits > 1 ? mapa_shared(slice, (uint32_t)owner) : 0u;
         const uint32_t remote_bar = splits > 1 ? mapa_shared(smem_u32(&bar_sums), (uint32_t)owner) : 0u;
         if (splits > 1 && threadIdx.x == 0)                 // every CTA's sums of this CTA's rows
@@ -866,7 +870,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           ok = ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutPeers);
           if (named_bar_any(1, 128, !ok)) return false;
           for (int i = (int)threadIdx.x; i < own_rows * tc.rows; i += 128) {
-            const int r = i % own_rows, tok = i / own_rows;
+            const int r = i & (own_rows - 1), tok = i >> own_bits;
             float v[kMats];
             #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
