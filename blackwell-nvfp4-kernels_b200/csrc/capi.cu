@@ -1351,7 +1351,8 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   // one token 16384 x 7168, 14.6 us with 6 slots, 17.2 with 4; with more than 8 tokens, or
   // many experts, the x slots need the rest (16 tokens 7168 x 16384 23.6 us with 216 KB, 25.8 with 160).
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
-  const int sums = p.splits > 1 ? kMats * p.group_rows * kBM * (int)sizeof(float) : 0;
+  const int send = self ? kGemvSend<true> : kGemvSend<false>;
+  const int sums = p.splits > 1 ? kMats * ((p.group_rows + send - 1) / send * send) * kBM * (int)sizeof(float) : 0;
   const int budget = (p.splits == 8 && p.group_rows <= 8 ? 112 : p.group_rows > 8 || (kMoe && !self) ? 216 : 160) * 1024;
   p.x_slots = self ? kGemvMaxXSlots : 4;
   p.w_slots = (budget - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;

@@ -423,15 +423,33 @@ __device__ __forceinline__ void tc_cp_32x128b_x4(uint32_t taddr, uint64_t s_desc
 
 // Store to shared memory of any CTA of the cluster, its bytes counted on an
 // mbarrier there: the data and the signal in one, no fence.
-__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr),
-               "r"(__float_as_uint(v)), "r"(cluster_bar)
+__device__ __forceinline__ void st_async(uint32_t cluster_addr, const float (&v)[1], uint32_t cluster_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(cluster_addr),
+               "f"(v[0]), "r"(cluster_bar)
                : "memory");
+}
+__device__ __forceinline__ void st_async(uint32_t cluster_addr, const float (&v)[4], uint32_t cluster_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                   cluster_addr),
+               "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "r"(cluster_bar)
+               : "memory");
+}
+__device__ __forceinline__ void lds_vec(uint32_t addr, float (&v)[1]) {
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void lds_vec(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Accumulator columns of two or four tokens.
+// Tokens of an epilogue step, which waits once for its loads; the columns behind
+// the last token's are other accumulators or scales, and not used.  And tokens of one
+// store between the CTAs of a cluster (16 tokens 7168 x 16384 19.2 us, 20.0 with stores of one
+// token; two tokens at once cost the self-expanding form 0.2 us).
+template <bool kSelf> constexpr int kGemvStep = kSelf ? 2 : 4;
+template <bool kSelf> constexpr int kGemvSend = kSelf ? 1 : 4;
+// Accumulator columns of a step.
 __device__ __forceinline__ void tmem_ld_terms(uint32_t taddr, uint32_t (&d)[16]) { tmem_ld_32x32b_x16(taddr, d); }
 __device__ __forceinline__ void tmem_ld_terms(uint32_t taddr, uint32_t (&d)[32]) { tmem_ld_32x32b_x32(taddr, d); }
 template <int N>
@@ -801,6 +819,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     uint32_t phase = 0, acc_phase = 0;
     int acc_buf = 0;
     auto finish = [&](int t, int index) -> bool {
+        constexpr int kStep = kGemvStep<kSelf>, kSend = kGemvSend<kSelf>;
         const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
         // before the wait: a load for each token in the loops below is 0.3 us a token
         if (row < tc.rows) {
@@ -816,49 +835,61 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
         // one K block: only the thread whose turn it was has written its accumulator
         const bool both = kDual || kb1 - kb0 > 1;
         const int only = index * (kb1 - kb0) & 1;
-        // sums of a sender in an owner's shared memory: [sender][matrix][token][row of the owner]
-        const uint32_t slice = sums_base + (uint32_t)((rank * kMats * tc.rows) * own_rows + (row & (own_rows - 1))) * 4u;
+        // sums of a sender in an owner's shared memory: [sender][matrix][token / kSend][row of the owner][token % kSend]
+        constexpr uint32_t kVec = 4u * kSend;
+        const int sends = (tc.rows + kSend - 1) / kSend;
+        const uint32_t slice = sums_base + (uint32_t)((rank * kMats * sends) * own_rows + (row & (own_rows - 1))) * kVec;
         const uint32_t remote = splits > 1 ? mapa_shared(slice, (uint32_t)owner) : 0u;
         const uint32_t remote_bar = splits > 1 ? mapa_shared(smem_u32(&bar_sums), (uint32_t)owner) : 0u;
         if (splits > 1 && threadIdx.x == 0)                 // every CTA's sums of this CTA's rows
-          mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * tc.rows * kBM) * 4u);
+          mbar_arrive_expect_tx(smem_u32(&bar_sums), (uint32_t)(kMats * sends * kBM) * kVec);
         auto out_at = [&](int tok) -> int64_t {              // where the token's row of this tile starts
           int64_t at;
           if constexpr (kMoe) at = (int64_t)s_row[index % 2][tok] * p.ldo;
           else at = (int64_t)tc.batch * p.out_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldo;
           return at + (int64_t)tc.row_block * kBM;
         };
-        // several tokens a step, which waits once for its loads; the columns behind the last token's
-        // are other accumulators' or scales, and not used
-        constexpr int kStep = kSelf ? 2 : 4;
         for (int t0 = 0; t0 < tc.rows; t0 += kStep) {
           uint32_t d[2][kStep * kGemvTerms];
           tmem_ld_terms(acc + (both ? 0 : only * n_pad) + t0 * kGemvTerms, d[0]);
           if (both) tmem_ld_terms(acc + n_pad + t0 * kGemvTerms, d[1]);
           tmem_ld_wait();
           tmem_terms_ready(d[0]), tmem_terms_ready(d[1]);
+          float v[2][kStep];
           #pragma unroll
           for (int i = 0; i < kStep; ++i) {
-            const int tok = t0 + i;
-            if (tok >= tc.rows) break;
-            const float back = s_back[index % 2][tok];
-            float v[2] = {0.f, 0.f};
-            #pragma unroll
-            for (int a = 0; a < 2; ++a)
-              if (a == 0 || both) {
-                v[a] = __uint_as_float(d[a][8 * i + 7]);
-                #pragma unroll
-                for (int j = 6; j >= 0; --j) v[a] = fmaf(v[a], 0.125f, __uint_as_float(d[a][8 * i + j]));
-                v[a] *= back;
-              }
-            if constexpr (!kDual) v[0] += v[1];
-            if (splits > 1) {
+            // without a branch for each token their chains of sums overlap (16 tokens 7168 x 16384 19.2 us, with
+            // it 20.0); sums behind the last token's are not stored
+            v[0][i] = v[1][i] = 0.f;
+            if (!kSelf || t0 + i < tc.rows) {
+              const float back = s_back[index % 2][t0 + i];
               #pragma unroll
-              for (int mat = 0; mat < kMats; ++mat)
-                st_async_f32(remote + (uint32_t)((mat * tc.rows + tok) * own_rows) * 4u, v[mat], remote_bar);
-            } else if (tc.row_block * kBM + row < p.n) {
-              store_out(p.out, p.out_dtype, out_at(tok) + row, kDual ? silu_gate_f32(v[0], v[1]) : v[0]);
+              for (int a = 0; a < 2; ++a)
+                if (a == 0 || both) {
+                  v[a][i] = __uint_as_float(d[a][8 * i + 7]);
+                  #pragma unroll
+                  for (int j = 6; j >= 0; --j) v[a][i] = fmaf(v[a][i], 0.125f, __uint_as_float(d[a][8 * i + j]));
+                  v[a][i] *= back;
+                }
             }
+            if constexpr (!kDual) v[0][i] += v[1][i];
+          }
+          if (splits > 1) {
+            #pragma unroll
+            for (int mat = 0; mat < kMats; ++mat)
+              #pragma unroll
+              for (int i = 0; i < kStep; i += kSend)
+                if (t0 + i < tc.rows) {
+                  float some[kSend];
+                  #pragma unroll
+                  for (int j = 0; j < kSend; ++j) some[j] = v[mat][i + j];
+                  st_async(remote + (uint32_t)((mat * sends + (t0 + i) / kSend) * own_rows) * kVec, some, remote_bar);
+                }
+          } else if (tc.row_block * kBM + row < p.n) {
+            #pragma unroll
+            for (int i = 0; i < kStep; ++i)
+              if (t0 + i < tc.rows)
+                store_out(p.out, p.out_dtype, out_at(t0 + i) + row, kDual ? silu_gate_f32(v[0][i], v[1][i]) : v[0][i]);
           }
         }
         // the accumulators may be overwritten
@@ -869,24 +900,32 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
         if (splits > 1) {
           ok = ctl.wait_cluster(smem_u32(&bar_sums), phase, kDevTimeoutPeers);
           if (named_bar_any(1, 128, !ok)) return false;
-          for (int i = (int)threadIdx.x; i < own_rows * tc.rows; i += 128) {
-            const int r = i & (own_rows - 1), tok = i >> own_bits;
-            float v[kMats];
+          for (int i = (int)threadIdx.x; i < own_rows * sends; i += 128) {
+            const int r = i & (own_rows - 1), send = i >> own_bits;
+            float v[kMats][kSend];
             #pragma unroll
             for (int mat = 0; mat < kMats; ++mat) {
-              float part[kGemvMaxSplits];                  // all loads before the first sum
+              float part[kGemvMaxSplits][kSend];           // all loads before the first sum
               #pragma unroll
               for (int s = 0; s < kGemvMaxSplits; ++s)
-                if (s < splits)
-                  part[s] = __uint_as_float(lds_u32(sums_base + (uint32_t)(((s * kMats + mat) * tc.rows + tok) * own_rows + r) * 4u));
-              v[mat] = part[0];
+                if (s < splits) lds_vec(sums_base + (uint32_t)(((s * kMats + mat) * sends + send) * own_rows + r) * kVec, part[s]);
               #pragma unroll
-              for (int s = 1; s < kGemvMaxSplits; ++s)
-                if (s < splits) v[mat] += part[s];
+              for (int j = 0; j < kSend; ++j) {
+                v[mat][j] = part[0][j];
+                #pragma unroll
+                for (int s = 1; s < kGemvMaxSplits; ++s)
+                  if (s < splits) v[mat][j] += part[s][j];
+              }
             }
             const int at = rank * own_rows + r;
-            if (tc.row_block * kBM + at < p.n)
-              store_out(p.out, p.out_dtype, out_at(tok) + at, kDual ? silu_gate_f32(v[0], v[kMats - 1]) : v[0]);
+            if (tc.row_block * kBM + at < p.n) {
+              #pragma unroll
+              for (int j = 0; j < kSend; ++j) {
+                const int tok = send * kSend + j;
+                if (tok < tc.rows)
+                  store_out(p.out, p.out_dtype, out_at(tok) + at, kDual ? silu_gate_f32(v[0][j], v[kMats - 1][j]) : v[0][j]);
+              }
+            }
           }
           if (t + clusters < tiles) {
             named_bar_sync(1, 128);                         // all of this CTA's rows are read: the next may come
