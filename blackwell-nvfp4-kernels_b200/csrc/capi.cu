@@ -1224,7 +1224,7 @@ GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
 // Clusters of `splits` CTAs that run at once.  Eight CTAs that need an SM each
 // (more than 8 tokens: see the shared memory below) find neighbouring SMs for about half of the
 // GPU: 16 tokens 2048 x 7168, 16 clusters, 14.9 us, and 9.6 with clusters of 4; 512 x 16384,
-// 4 clusters, 10.0 us and 11.8.
+// 4 clusters, 9.3 us and 10.8.
 int gemv_clusters(int splits, int group_rows, int num_sms) {
   return splits == 8 && group_rows > 8 ? (num_sms + 15) / 16 : num_sms / splits;
 }
@@ -1232,9 +1232,8 @@ int gemv_clusters(int splits, int group_rows, int num_sms) {
 // CTAs of a cluster that share a tile's K: the count (a power of two, so that
 // the 128 rows divide) with the fewest K blocks on the busiest CTA.  The exchange of a
 // tile's sums counts as three K blocks (about 1 us).  Measured, us with 1 / 2 / 4 / 8 CTAs, one
-// token: 512 x 1024 4.7 / 5.0 / 5.0 / 5.0, 2048 x 7168 14.7 / 10.8 / 7.9 / 6.8, 4096 x 14336 26.2 / 17.6 /
-// 12.8 / 11.9, 16384 x 7168 17.0 / 17.7 / 18.0 / 25.7; 16 tokens 7168 x 16384 28.6 / 24.2 / 31.0 / 51.4
-// (with an epilogue 3 us slower than now).
+// token: 512 x 1024 4.2 / 4.4 / 4.4 / -, 2048 x 7168 10.8 / 8.0 / 6.3 / 6.1, 4096 x 14336 17.2 / 12.1 / 9.9 /
+// 10.4, 16384 x 7168 14.2 / 14.5 / 25.6 / 29.5; 16 tokens 7168 x 16384 25.3 / 19.4 / 22.7 / 28.4.
 int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
   int best = 1;
   long long least = 0;
@@ -1248,8 +1247,9 @@ int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
 
 // Whether gemv_kernel expands x itself: one launch less, but its eight warps
 // take about 1 us for 8 K blocks of a token.  Measured, us with / without: one token 512 x
-// 1024 4.6 / 5.4, 4096 x 14336 (14 K blocks a CTA) 10.9 / 11.5, 16384 x 7168 (28) 14.6 / 15.3; four
-// tokens 14336 x 4096 (16) 21 / 12.3.  8 experts of one token 4096 x 1536 7.1 / 9.9.
+// 1024 4.2 / 5.2, 4096 x 14336 (14 K blocks a CTA) 9.8 / 11.2, 16384 x 7168 (28) 14.2 / 15.3; two tokens 8192 x
+// 8192 (32) 10.9 / 12.1, 16384 x 7168 (56) 16.4 / 15.6; four tokens 14336 x 4096 (64) 21 / 12.  8 experts
+// of a token, gated, 2048 x 7168 25.2 / 29.7; 2 experts of a token 4096 x 1536 6.5 / 9.5.
 bool gemv_expands_itself(int x_dtype, bool x_vec, int rows, int span) {
   return x_dtype != kDtF32 && x_vec && rows <= kGemvSelfTokens && rows * span <= 32;
 }
@@ -1347,9 +1347,10 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.status = d->status;
   p.wait_limit = wait_limit_cycles();
   // Shared memory.  Clusters of 8 CTAs find room for all of their SMs only when two
-  // CTAs fit on one (2048 x 7168: 6.8 us with 112 KB, 12.7 with 160).  Otherwise more weight slots pay:
-  // one token 16384 x 7168, 14.6 us with 6 slots, 17.2 with 4; with more than 8 tokens, or
-  // many experts, the x slots need the rest (16 tokens 7168 x 16384 23.6 us with 216 KB, 25.8 with 160).
+  // CTAs fit on one (2048 x 7168: 6.0 us with 112 KB, 10.8 with 160).  Otherwise more weight slots pay:
+  // one token 16384 x 7168 14.2 us with 6 slots, 16.6 with 4; with more than 8 tokens, or
+  // many experts, the x slots need the rest (16 tokens 7168 x 16384 19.4 us with 216 KB, 21.6 with 160; 64
+  // rows of experts 7168 x 2048 59.8 and 60.5), with fewer they do not (5 tokens 4099 x 7168 9.6 and 9.4).
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
   const int send = self ? kGemvSend<true> : kGemvSend<false>;
   const int sums = p.splits > 1 ? kMats * ((p.group_rows + send - 1) / send * send) * kBM * (int)sizeof(float) : 0;
