@@ -127,7 +127,7 @@ def gemv(x: torch.Tensor, w: Weights, out: torch.Tensor | None = None,
     """x . Wᵀ for x [M, K] (or [L, M, K], L matrices): [M, N] (or [L, M, N]) in
     ``out_dtype`` (x's type by default; fp16, bf16 or fp32), one rounding of an
     fp32 sum.  ``out``: written and returned instead of a new tensor; its rows may
-    be strided.  Meant for M <= 16; every 16 further tokens (8 in fp32) read the
+    be strided; it must not overlap x or the weights.  Meant for M <= 16; every 16 further tokens (8 in fp32) read the
     weights again."""
     return _run(x, w, None, out, out_dtype)
 

@@ -66,7 +66,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
              residual_out: torch.Tensor | None = None):
     """(y, h) for x [rows, K], K <= 32768; y [rows, K] in ``out_dtype`` (x's type by
     default).  x, weight, residual and y may each be float16, bfloat16 or float32;
-    ``residual_out`` may be ``residual`` itself (then updated in place)."""
+    ``residual_out`` may be ``residual`` itself and ``out`` may be ``x`` (then updated
+    in place); nothing else may overlap."""
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if out is None:

@@ -199,8 +199,9 @@ size_t nvfp4_moe_table_bytes(int num_experts);
 
 /* h = x + residual (rounded to the residual's type; h = x when residual is NULL),
  * y = h / sqrt(mean(h^2) + eps) * weight over the K columns of each row, in one
- * pass.  h may be the residual itself.  The sum of squares and the root are fp64, h *
- * r and the product with the weight are rounded to fp32 one after the other.
+ * pass.  h may be the residual itself and a PLAIN y may be x (the same type and stride);
+ * nothing else overlaps.  The sum of squares and the root are fp64, h * r and the product
+ * with the weight are rounded to fp32 one after the other.
  *   PLAIN  y in y_dtype
  *   FP8    scale = amax/448 over `group` columns (32, 64 or 128, dividing K; 0: the
  *          row), y = e4m3_rne(y/scale), scales [rows][K/group]; zeros under a

@@ -236,6 +236,54 @@ def test_gemv_on_another_device():
     check(V.gemv(x.to("cuda:1"), other), *products(x, dense[0]))
 
 
+def test_gemv_broadcast_batches_and_out_batches_apart():
+    l, m, n, k = 3, 4, 140, 384
+    w, dense = make_weights(n, k, seed=12, l=l)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(1)).half().cuda()
+    big = torch.full((l, m + 2, n + 3), float("nan"), dtype=torch.float32, device="cuda")
+    got = V.gemv(x[None].expand(l, m, k), w, out=big[:, 1:1 + m, :n])
+    for b in range(l):
+        check(got[b], *products(x, dense[b]))
+    assert int(torch.isnan(big).sum()) == big.numel() - l * m * n
+
+
+def test_gemv_weights_past_32_bit_offsets():
+    """More than 2^31 bytes of weights: the last row blocks against their own products."""
+    n, k, m = 70016, 65536, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    b = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8, device="cuda")
+    sf = torch.randint(0x20, 0x40, (n // 128, k // 64, 32, 4, 4), generator=g, dtype=torch.uint8, device="cuda")
+    x = torch.randn(m, k, generator=g, device="cuda").bfloat16()
+    got = {rows: V.gemv(x[:rows], V.Weights(b, sf), out_dtype=torch.float32) for rows in (1, m)}
+    for blk in (0, n // 128 - 1):
+        rows = slice(128 * blk, 128 * blk + 128)
+        plain = sf[blk].permute(2, 1, 0, 3).reshape(128, k // 16).cpu().numpy()
+        dense = O.dequantize(b[rows].cpu().numpy(), plain).astype(np.float64)
+        y, bound = products(x, dense)
+        for r, out in got.items():
+            check(out[:, rows], y[:r], bound[:r])
+    assert _lib.device_status() == 0
+
+
+def test_gemv_two_captured_graphs_at_once():
+    """Each graph's workspace is its own: replays of both on two streams give what the calls give."""
+    w, _ = make_weights(1300, 2560, seed=2)
+    xs = [torch.randn(m, 2560, device="cuda").bfloat16() for m in (5, 11)]
+    graphs = [_capture(lambda x=x: V.gemv(V.gemv(x, w)[:, :64].repeat(1, 40), w)) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for seed in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)).bfloat16())
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, (graph, _) in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for x, (_, out) in zip(xs, graphs):
+            assert torch.equal(out, V.gemv(V.gemv(x, w)[:, :64].repeat(1, 40), w))
+
+
 # ---------------------------------------------------------------------------
 # experts
 # ---------------------------------------------------------------------------
@@ -297,6 +345,37 @@ def test_moe_gemv_out_rows_apart_and_one_choice_vector():
     for p in range(6):
         check(got[p:p + 1], *products(x[p][None], d[int(ids[p])]))
     assert bool(torch.isnan(big[:, :16]).all()) and bool(torch.isnan(big[:, 112:]).all())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_moe_gemv_unaligned_x_and_strided_choices(dtype):
+    w, d = make_experts(6, 160, 448, seed=20)
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randn(5, 470, generator=g).to(TYPES[dtype]).cuda()
+    ids = torch.randint(0, 6, (3, 5), generator=g, dtype=torch.int32).cuda().T
+    for off in (0, 8, 3):
+        x = wide[:, off:off + 448]
+        got = moe.gemv(x, ids, w, out_dtype=torch.float32)
+        for p, ex in enumerate(ids.reshape(-1).tolist()):
+            check(got[p:p + 1], *products(x[p // 3][None], d[ex]))
+
+
+def test_moe_gemv_non_finite_tokens_are_nan_and_leave_the_others():
+    w, d = make_experts(3, 140, 512, seed=30)
+    for tokens in (3, 30):
+        x = torch.randn(tokens, 512, generator=torch.Generator().manual_seed(1)).half()
+        ids = torch.zeros(tokens, 2, dtype=torch.int32)        # all of them in the groups of one expert
+        ids[:, 1] = 2
+        y = [products(x, d[0]), products(x, d[2])]
+        x[1, 300] = float("inf")
+        got = moe.gemv(x.cuda(), ids.cuda(), w)
+        for t in range(tokens):
+            for j in range(2):
+                row = got[2 * t + j][None]
+                if t == 1:
+                    assert bool(torch.isnan(row).all())
+                else:
+                    check(row, y[j][0][t:t + 1], y[j][1][t:t + 1])
 
 
 # ---------------------------------------------------------------------------

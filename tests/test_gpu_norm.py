@@ -136,6 +136,27 @@ def test_rms_norm_in_place_strided_and_unaligned():
         assert all(a.data_ptr() == b.data_ptr() for a, b in zip(first, again))
 
 
+def test_rms_norm_onto_its_input():
+    x = torch.randn(20, 3000, generator=torch.Generator().manual_seed(3)).half().cuda()
+    w = torch.rand(3000, generator=torch.Generator().manual_seed(4)).half().cuda()
+    want, _ = norm.rms_norm(x, w)
+    y, h = norm.rms_norm(x, w, out=x)
+    assert y is x and h is x and torch.equal(x, want)
+
+
+def test_rms_norm_past_32_bit_offsets():
+    rows, k = 66000, 32768
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    (q, s), _ = norm.rms_norm_fp8(x, w)
+    (packed, sf, _), _ = norm.rms_norm_nvfp4(x, w)
+    for part in (slice(0, 2), slice(rows - 2, rows)):
+        (q2, s2), _ = norm.rms_norm_fp8(x[part].clone(), w)
+        (packed2, sf2, _), _ = norm.rms_norm_nvfp4(x[part].clone(), w)
+        for a, b in ((q[part], q2), (s[part], s2), (packed[part], packed2), (sf[part], sf2)):
+            assert torch.equal(a.view(torch.uint8).cpu(), b.view(torch.uint8).cpu())
+
+
 def test_rms_norm_special_rows():
     """Zero rows, tiny and huge ones, infinities and NaN, and a gain that is not finite."""
     k = 256
