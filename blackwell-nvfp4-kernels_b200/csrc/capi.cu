@@ -1221,19 +1221,22 @@ GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
   return s;
 }
 
-// Clusters of `splits` CTAs that run at once.  Eight CTAs that need an SM each
-// (more than 8 tokens: see the shared memory below) find neighbouring SMs for about half of the
-// GPU: 16 tokens 2048 x 7168, 16 clusters, 14.9 us, and 9.6 with clusters of 4; 512 x 16384,
-// 4 clusters, 9.3 us and 10.8.
+// Clusters of eight CTAs find neighbouring SMs for about half of the GPU when each
+// CTA needs an SM; all of it when two CTAs fit on one, with half of the slots.  Few tokens are better
+// off with all clusters (one token 2048 x 7168, 16 clusters, 6.0 us and 6.2 with clusters of 4; two tokens
+// 6.2 and 6.7), unless there are no more than fit alone (1024 x 16384, 8 clusters, 7.1 and 6.6 us); three
+// and more tokens with clusters of 4 (8 tokens 2048 x 7168 9.7 and 8.2 us, three 8.8 and 7.8).
+int gemv_lone_clusters(int num_sms) { return (num_sms + 15) / 16; }
+// Clusters of `splits` CTAs that run at once.
 int gemv_clusters(int splits, int group_rows, int num_sms) {
-  return splits == 8 && group_rows > 8 ? (num_sms + 15) / 16 : num_sms / splits;
+  return splits == 8 && group_rows > kGemvSelfTokens ? gemv_lone_clusters(num_sms) : num_sms / splits;
 }
 
 // CTAs of a cluster that share a tile's K: the count (a power of two, so that
 // the 128 rows divide) with the fewest K blocks on the busiest CTA.  The exchange of a
 // tile's sums counts as three K blocks (about 1 us).  Measured, us with 1 / 2 / 4 / 8 CTAs, one
-// token: 512 x 1024 4.2 / 4.4 / 4.4 / -, 2048 x 7168 10.8 / 8.0 / 6.3 / 6.1, 4096 x 14336 17.2 / 12.1 / 9.9 /
-// 10.4, 16384 x 7168 14.2 / 14.5 / 25.6 / 29.5; 16 tokens 7168 x 16384 25.3 / 19.4 / 22.7 / 28.4.
+// token: 512 x 1024 4.2 / 4.4 / 4.4 / -, 2048 x 7168 10.8 / 8.0 / 6.3 / 6.0, 4096 x 14336 17.2 / 12.1 / 9.8 /
+// 10.4, 16384 x 7168 13.6 / 14.5 / 25.6 / 29.5; 16 tokens 7168 x 16384 25.3 / 19.4 / 22.7 / 28.4.
 int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
   int best = 1;
   long long least = 0;
@@ -1247,9 +1250,9 @@ int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
 
 // Whether gemv_kernel expands x itself: one launch less, but its eight warps
 // take about 1 us for 8 K blocks of a token.  Measured, us with / without: one token 512 x
-// 1024 4.2 / 5.2, 4096 x 14336 (14 K blocks a CTA) 9.8 / 11.2, 16384 x 7168 (28) 14.2 / 15.3; two tokens 8192 x
-// 8192 (32) 10.9 / 12.1, 16384 x 7168 (56) 16.4 / 15.6; four tokens 14336 x 4096 (64) 21 / 12.  8 experts
-// of a token, gated, 2048 x 7168 25.2 / 29.7; 2 experts of a token 4096 x 1536 6.5 / 9.5.
+// 1024 4.2 / 5.2, 4096 x 14336 (14 K blocks a CTA) 9.8 / 11.2, 16384 x 7168 (28) 13.6 / 15.3; two tokens 8192 x
+// 8192 (32) 10.6 / 12.1, 16384 x 7168 (56) 16.4 / 15.6; four tokens 14336 x 4096 (64) 21 / 12.  8 experts
+// of a token, gated, 2048 x 7168 24.6 / 29.7; 2 experts of a token 4096 x 1536 6.4 / 9.5.
 bool gemv_expands_itself(int x_dtype, bool x_vec, int rows, int span) {
   return x_dtype != kDtF32 && x_vec && rows <= kGemvSelfTokens && rows * span <= 32;
 }
@@ -1346,31 +1349,33 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.image = ws + sp.image;
   p.status = d->status;
   p.wait_limit = wait_limit_cycles();
-  // Shared memory.  Clusters of 8 CTAs find room for all of their SMs only when two
-  // CTAs fit on one (2048 x 7168: 6.0 us with 112 KB, 10.8 with 160).  Otherwise more weight slots pay:
-  // one token 16384 x 7168 14.2 us with 6 slots, 16.6 with 4; with more than 8 tokens, or
-  // many experts, the x slots need the rest (16 tokens 7168 x 16384 19.4 us with 216 KB, 21.6 with 160; 64
-  // rows of experts 7168 x 2048 59.8 and 60.5), with fewer they do not (5 tokens 4099 x 7168 9.6 and 9.4).
+  // Shared memory.  Two CTAs of many clusters of 8 share an SM (see above; 2048 x 7168 10.8 us
+  // with 160 KB).  Otherwise bytes on their way pay: one token 16384 x 7168 16.6 / 14.1 / 13.6 / 13.8 us with
+  // 4 / 6 / 8 / 12 weight slots; 16 tokens 7168 x 16384 21.6 us with 160 KB, 19.3 with 216; 5 tokens 7168 x 16384
+  // 17.8 and 17.1 (with 6 x slots, 17.2 with 4; of a few rows of many experts, 64 of 7168 x 2048, 60.3
+  // and 59.2).  The numbers of slots are even: see gemv_kernel.
   const int x_bytes = p.group_rows * kGemvTokenBytes + kGemvXSfBytes;
   const int send = self ? kGemvSend<true> : kGemvSend<false>;
   const int sums = p.splits > 1 ? kMats * ((p.group_rows + send - 1) / send * send) * kBM * (int)sizeof(float) : 0;
-  const int budget = (p.splits == 8 && p.group_rows <= 8 ? 112 : p.group_rows > 8 || (kMoe && !self) ? 216 : 160) * 1024;
-  p.x_slots = self ? kGemvMaxXSlots : 4;
+  const bool shared_sm = p.splits == 8 && p.group_rows <= kGemvSelfTokens && tiles > gemv_lone_clusters(d->num_sms);
+  const int budget = (shared_sm ? 112 : 216) * 1024;
+  p.x_slots = self ? kGemvMaxXSlots : kMoe || p.group_rows > 8 ? 4 : 6;
   p.w_slots = (budget - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
   if (p.w_slots > kGemvMaxWSlots) p.w_slots = kGemvMaxWSlots;
-  if (self && p.w_slots > 6) p.w_slots = 6;             // TMEM: 256 columns
+  if (self && p.w_slots > 8) p.w_slots = 8;
   p.w_slots &= ~1;
   const int smem = 1024 + p.w_slots * kGemvWBytes + p.x_slots * x_bytes + sums;
   // TMEM: two accumulators (twice where there is room) and the slots' scales
-  // (two CTAs share an SM only under the 112 KB budget: at most 4 weight slots and 8 tokens, 256
+  // (two CTAs share an SM only under the 112 KB budget: at most 4 weight slots and 2 tokens, 256
   // columns each, so that neither waits for columns of the other while its cluster waits for it)
   const int n_pad = (p.group_rows * kGemvTerms + 15) / 16 * 16, sf_cols = kGemvSfCols * p.w_slots;
   p.acc_bufs = 4 * n_pad + sf_cols <= 256 ? 2 : 2 * n_pad + sf_cols <= 256 ? 1 : 4 * n_pad + sf_cols <= 512 ? 2 : 1;
   const int cols = p.acc_bufs * 2 * n_pad + sf_cols;
-  if (p.w_slots < 2 || cols > (self ? 256 : 512) || (self && p.acc_bufs != 2))
+  if (p.w_slots < 2 || cols > 512 || (self && p.acc_bufs != 2))
     return fail(NVFP4_ERR_SHAPE, "%d weight slots, %d TMEM columns", p.w_slots, cols);
-  const int base = 32 + (kDual ? 6 : 0) + (kMoe ? 3 : 0);
-  if (self) return launch_gemv<kDual, kMoe, true, 256>(d, base, p, smem, tiles, stream);
+  const int base = 32 + (kDual ? 8 : 0) + (kMoe ? 4 : 0);
+  if (self && cols <= 256) return launch_gemv<kDual, kMoe, true, 256>(d, base, p, smem, tiles, stream);
+  if (self) return launch_gemv<kDual, kMoe, true, 512>(d, base + 3, p, smem, tiles, stream);
   if (cols <= 256) return launch_gemv<kDual, kMoe, false, 256>(d, base + 1, p, smem, tiles, stream);
   return launch_gemv<kDual, kMoe, false, 512>(d, base + 2, p, smem, tiles, stream);
 }

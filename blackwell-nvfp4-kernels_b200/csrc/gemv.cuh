@@ -410,7 +410,7 @@ constexpr int kGemvWBytes = kBM * kBK / 2 + kSfStageBytes;   // a weight slot: 1
 constexpr int kBMBits = 7;
 static_assert(1 << kBMBits == kBM, "rows of a block");
 constexpr int kGemvSfCols = 32;          // TMEM columns of a weight slot: its scales and x's
-constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // x slots a power of two
+constexpr int kGemvMaxWSlots = 12, kGemvMaxXSlots = 8;        // even; 8 x slots where the kernel expands x
 constexpr int kGemvSelfTokens = 2;       // largest group that gemv_kernel expands itself
 constexpr int kGemvSelfPairs = 32;       // and the most rows of an expert call
 // warps: epilogue 0-3, expansion 0-7 (without it x copies: 4), then weights, two for the MMAs
@@ -497,14 +497,14 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSma
 // shared memory: each CTA owns 128 / splits rows, gets the others' sums for them and
 // adds them in the order of the CTAs.
 //
-// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 14.2 us;
-// the same ring without any MMA, all of the GPU reading 66 MB of other data, takes 14.1, plain 32-byte
-// loads 12.4 (10.1 us at the rate of a long copy: what is short here is the time).  The
-// gated pair 14336 x 4096 (66 MB) 14.5 us, 8 experts of a token 2048 x 7168 (132 MB) 25.1 (ring 23.8), 64
-// rows of experts 7168 x 2048 (348 MB) 59.8 us, 5.8 TB/s.  Smaller calls are bound by the chain from the
-// end of the work before to the first product and from the last to the output, about 4 us: 4.5 us for
-// 1001 x 1536 (0.9 MB).  Each token adds 0.1 us of epilogue and its part of x: 16 tokens
-// 7168 x 16384 19.3 us, one 15.4.
+// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 13.6 us (4.9
+// TB/s); a ring of 90 KB without any MMA, all of the GPU reading 66 MB of other data, takes 14.1, plain
+// 32-byte loads 12.4 (10.1 us at the rate of a long copy: what is short here is the time).  The
+// gated pair 14336 x 4096 (66 MB) 14.3 us, 8 experts of a token, gated, 2048 x 7168 (132 MB) 24.6 (the
+// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 59.4 us, 5.9 TB/s.  Smaller calls are bound by the
+// chain from the end of the work before to the first product and from the last to the output, about
+// 4 us: 4.5 us for 1001 x 1536 (0.9 MB).  More tokens cost the expansion, 0.1 us of epilogue each
+// and room for fewer weights on their way: 7168 x 16384 14.6 us for one, 19.3 for 16.
 template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
 __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __grid_constant__ GemvParams p) {
   constexpr int kMats = kDual ? 2 : 1;
@@ -669,8 +669,9 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     // barrier check costs its thread 30 to 100 cycles, and one thread's 770 cycles for a
     // K block (two waits, eight copies, four MMAs, two commits; measured) were as long as
     // the block takes to arrive.  They take the weight slots in turn: gate and up, or even and
-    // odd K blocks, whose sums the epilogue adds.  (The number of slots is even, so that a
-    // slot is always the same thread's and its phases are waited for one after the other.)
+    // odd K blocks, whose sums the epilogue adds.  (The numbers of slots, x's too, are even, so that
+    // a slot is always the same thread's and its phases are waited for one after the other: a thread that
+    // tested a phase the other had not waited for could take the one before for it.)
     griddep_wait();                                       // nothing to do before; and no polling beside a kernel at work
     if (elect_one()) {
       const int me = warp - kMmaWarp;
