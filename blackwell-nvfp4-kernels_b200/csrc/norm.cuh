@@ -7,7 +7,8 @@
 // and y as
 //   kNormPlain  fp16, bf16 or fp32;
 //   kNormFp8    e4m3 with one fp32 scale for each `group` columns (or the whole
-//               row): s = amax / 448, q = e4m3_rne(y / s), all zero when s is 0;
+//               row): s = amax / 448, q = e4m3_rne(y / s) (from h * weight: the rounding of
+//               r does not move a code), all zero when s is 0;
 //   kNormNvfp4  e2m1 + e4m3 scales per 16 in the layouts the GEMMs read, by the
 //               rules of quantize.cuh.
 //
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
   } else {
     r = (float)rsqrt(fma(sum, p.inv_k, p.eps));
   }
-  auto values = [&](int i, float (&v)[8]) {               // y of chunk i
+  auto values = [&](int i, float (&v)[8], float r) {      // h r weight of chunk i
     float w[8];
     if constexpr (NV > 1) wt = norm_load8<kVec>(p.weight, w_dtype, col_of(i), p.k - col_of(i));
     widen8(wt, w_dtype, w);
@@ -321,17 +322,24 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float v[8];
-      values(i, v);
+      values(i, v, r);
       norm_store8<kVec>(p.y, p.y_dtype, (int64_t)row * p.ldy + col_of(i), p.k - col_of(i), norm_round(v, p.y_dtype));
     }
   } else if constexpr (kOut == kNormFp8 || kOut == kNormFp8Row) {
-    // chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then
+    // With r = r2 rho, r2 a power of two, v = h r2 weight is exact for 16-bit types and as far from
+    // over- and underflow as y = v rho.  y / s = v (448 / largest v): two roundings, where y, its
+    // largest, s and the quotient would have six, each of which can move a code that is near a border.
+    // Chunks past the row's end hold 0 * r * 0: NaN when r is, as the whole row is then.
+    const uint32_t r_bits = __float_as_uint(r);
+    const bool r_normal = r >= 1.1754944e-38f && r <= 3.402823466e38f;
+    const float r2 = r_normal ? __uint_as_float(r_bits & 0x7f800000u) : r;
+    const float rho = r_normal ? __uint_as_float((r_bits & 0x7fffffu) | 0x3f800000u) : 1.f;
     float row_top = 0.f;
     if constexpr (kOut == kNormFp8Row) {
       #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float v[8];
-        values(i, v);
+        values(i, v, r2);
         row_top = max_nan(row_top, largest_of(v));
       }
       #pragma unroll
@@ -347,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float v[8];
-      values(i, v);
+      values(i, v, r2);
       float top = row_top;
       if constexpr (kOut == kNormFp8) {
         top = largest_of(v);
@@ -356,15 +364,24 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
           if (8 * o < 1 << p.group_bits) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
       const int col = col_of(i), left = p.k - col;
-      // 448 = 1.75 * 2^8: a mantissa of the exhaustive proof in quantize.cuh; y and s between
-      // 2^-90 and 2^120 where it matters
-      float s = div_by_scale(top, 448.f, 1.f / 448.f);
-      const bool fast = top >= 3.308722e-24f /* 2^-78 */ && top <= 8.507059e37f /* 2^126 */ &&
-                        (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu;
-      if (!fast) s = __fdiv_rn(top, 448.f);
+      // Markstein's theorem (see div_by_scale) for / 448 = 1.75 * 2^8, a mantissa of the exhaustive
+      // proof in quantize.cuh, and for 448 / top unless top's mantissa is all ones; numbers between 2^-90 and
+      // 2^126 where it matters
+      const float y_top = __fmul_rn(top, rho);
+      const bool fast = top >= 3.308722e-24f /* 2^-78 */ && top <= 4.253530e37f /* 2^125 */ &&
+                        (__float_as_uint(top) & 0x7fffffu) != 0x7fffffu;
+      const float s = fast ? div_by_scale(y_top, 448.f, 1.f / 448.f) : __fdiv_rn(y_top, 448.f);
       uint32_t code[2] = {0u, 0u};
       if (s != 0.f) {
-        norm_divide(v, s, fast);
+        if (fast) {
+          const float c = div_by_scale(448.f, top, __frcp_rn(top));
+          #pragma unroll
+          for (int e = 0; e < 8; e += 2) unpack2(mul2(pack2(v[e], v[e + 1]), pack2(c, c)), v[e], v[e + 1]);
+        } else {
+          #pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(v[e], rho);
+          norm_divide(v, s, false);
+        }
         #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3);
@@ -392,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAny
     #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float v[8];
-      values(i, v);
+      values(i, v, r);
       const int col = col_of(i);
       float amax = largest_of(v);
       amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));

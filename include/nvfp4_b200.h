@@ -204,8 +204,9 @@ size_t nvfp4_moe_table_bytes(int num_experts);
  * with the weight are rounded to fp32 one after the other.
  *   PLAIN  y in y_dtype
  *   FP8    scale = amax/448 over `group` columns (32, 64 or 128, dividing K; 0: the
- *          row), y = e4m3_rne(y/scale), scales [rows][K/group]; zeros under a
- *          zero scale, a NaN scale for a group that holds a NaN
+ *          row), y = e4m3_rne(y/scale), the quotient off by at most 1.5 units in fp32's
+ *          last place (of h * weight, without r), scales [rows][K/group]; zeros under
+ *          a zero scale, a NaN scale for a group that holds a NaN
  *   NVFP4  y quantised as nvfp4_quantize does (K % 64 == 0): packed in y, atoms
  *          in sf_perm (padding rows zero), plain scales in sf_plain unless NULL;
  *          a NaN scale for 16 columns that hold a NaN
