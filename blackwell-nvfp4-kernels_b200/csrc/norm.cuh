@@ -220,7 +220,7 @@ __device__ __forceinline__ void norm_divide(float (&v)[8], float s, bool fast) {
 // One CTA for each row (chunks of 8 elements, chunk c = thread + i * threads,
 // i < NV); kNormNvfp4: CTAs past the rows clear the padding rows of the last
 // block's scale atoms.  kVec: every 8 elements of every tensor are 16-byte aligned
-// and K % 8 == 0.  kWide: h is fp32.
+// and K % 8 == 0.
 //
 // Bound: 7 bytes an element at 16 bits (fp8), 63 us of 8192 x 7168 at the rate of a copy; the
 // kernel takes 66.4 (6.2 TB/s), its instructions (28 an element) 72 % of the issue slots.  16-bit
