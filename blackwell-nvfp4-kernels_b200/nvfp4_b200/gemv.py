@@ -65,13 +65,8 @@ def _rows_last(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _new(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A contiguous tensor (the cheapest of torch's allocating calls)."""
-    strides, n = [1] * len(shape), 1
-    for i in range(len(shape) - 1, 0, -1):
-        n *= shape[i]
-        strides[i - 1] = n
-    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+# the cheapest of torch's allocating calls with a shape of its own
+_empty = torch.empty_strided
 
 
 def _launch(fn, device, args) -> None:
@@ -95,7 +90,7 @@ def _run(x, w, w2, out, out_dtype):
     x = _rows_last(x)
     want = (l, m, n) if dims == 3 else (m, n)
     if out is None:
-        out = _new(want, out_dtype or x.dtype, x.device)
+        out = _empty(want, (n, 1) if dims == 2 else (m * n, n, 1), dtype=out_dtype or x.dtype, device=x.device)
         if out.dtype not in DTYPES:
             raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
     elif (tuple(out.shape) != want or out.dtype not in DTYPES or out.device != x.device
@@ -114,7 +109,7 @@ def _run(x, w, w2, out, out_dtype):
         with torch.cuda.device(w.device):
             size = lib.nvfp4_gemv_workspace_bytes(code, aligned, m, n, k, l)
         w.space[(m, code, aligned)] = size
-    space = _new((size,), torch.uint8, x.device) if size else None
+    space = _empty((size,), (1,), dtype=torch.uint8, device=x.device) if size else None
     _launch(lib.nvfp4_gemv, x.device, (
         px, code, xs[-2], xb, *w.ptrs, *(w2.ptrs if w2 is not None else (None, None)), out.data_ptr(),
         DTYPES[out.dtype], os_[-2] if os_[-2] > n else n, ob, m, n, k, l,

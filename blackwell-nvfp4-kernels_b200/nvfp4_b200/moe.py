@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .dual_gemm import on_device
-from .gemv import DTYPES, _launch, _new, _rows_last
+from .gemv import DTYPES, _empty, _launch, _rows_last
 
 
 @dataclass
@@ -231,7 +231,7 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
         raise ValueError(f"x {tuple(x.shape)} is neither [{tokens}, {k}] nor [{rows}, {k}]")
     x, ids = _rows_last(x), ids.contiguous()
     if out is None:
-        out = _new((rows, n), out_dtype or x.dtype, x.device)
+        out = _empty((rows, n), (n, 1), dtype=out_dtype or x.dtype, device=x.device)
         if out.dtype not in DTYPES:
             raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
     elif (tuple(out.shape) != (rows, n) or out.dtype not in DTYPES or out.device != x.device
@@ -247,7 +247,7 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
     if size is None:
         size = w.space[(tokens, topk, code, aligned)] = lib.nvfp4_moe_gemv_workspace_bytes(code, aligned, tokens,
                                                                                           topk, k)
-    space = _new((size,), torch.uint8, x.device) if size else None
+    space = _empty((size,), (1,), dtype=torch.uint8, device=x.device) if size else None
     _launch(lib.nvfp4_moe_gemv, x.device, (
         px, code, ldx, x.shape[0] == rows and topk > 1, ids.data_ptr(), tokens, topk, w.table().data_ptr(),
         w2.table().data_ptr() if w2 is not None else None, len(w), out.data_ptr(), DTYPES[out.dtype],

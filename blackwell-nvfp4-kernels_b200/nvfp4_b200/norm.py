@@ -16,7 +16,14 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .gemv import DTYPES, _launch, _new, _rows_last
+from .gemv import DTYPES, _launch, _rows_last
+
+_empty, _empty_like = torch.empty_strided, torch.empty_like
+
+
+def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of x's shape (empty_like is the cheapest call, for contiguous x)."""
+    return _empty_like(x, dtype=dtype) if x.is_contiguous() else _empty(x.shape, (x.shape[1], 1), dtype=dtype, device=x.device)
 
 
 def _check(x, weight, residual, residual_out):
@@ -40,7 +47,7 @@ def _check(x, weight, residual, residual_out):
         raise ValueError(f"residual must be float16, bfloat16 or float32 [{rows}, {k}] on {device}")
     h = residual_out
     if h is None:
-        h = _new((rows, k), residual.dtype, device)
+        h = _like(residual, residual.dtype)
     elif (h.shape != shape or h.dtype != residual.dtype or h.device != device
           or (h.stride(1) != 1 and k > 1) or (rows > 1 and h.stride(0) < k)):
         raise ValueError(f"residual_out must be {residual.dtype} [{rows}, {k}], rows apart, on {device}")
@@ -71,7 +78,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if out is None:
-        out = _new((rows, k), out_dtype or x.dtype, x.device)
+        out = _like(x, out_dtype or x.dtype)
         if out.dtype not in DTYPES:
             raise ValueError(f"out_dtype {out_dtype} is none of float16, bfloat16 and float32")
     elif (tuple(out.shape) != (rows, k) or out.dtype not in DTYPES or out.device != x.device
@@ -99,8 +106,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
         raise ValueError(f"K={k} must be a multiple of the group ({group})")
     groups = 1 if group is None else k // group
     if out is None:
-        q = _new((rows, k), torch.float8_e4m3fn, x.device)
-        scales = _new((rows, groups), torch.float32, x.device)
+        q = _like(x, torch.float8_e4m3fn)
+        scales = _empty((rows, groups), (groups, 1), dtype=torch.float32, device=x.device)
     else:
         q, scales = out
         if (tuple(q.shape) != (rows, k) or tuple(scales.shape) != (rows, groups)
@@ -134,9 +141,9 @@ def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
                     or any(a != b for a, b, n in zip(t.stride(), strides, shape) if n > 1)):
                 raise ValueError("out does not match: pass the three tensors an earlier call returned")
     else:
-        packed = torch.empty_strided(*views[0], dtype=torch.float4_e2m1fn_x2, device=x.device)
-        sf = torch.empty_strided(*views[1], dtype=torch.float8_e4m3fn, device=x.device)
-        sf_perm = torch.empty_strided(*views[2], dtype=torch.float8_e4m3fn, device=x.device)
+        packed = _empty(*views[0], dtype=torch.float4_e2m1fn_x2, device=x.device)
+        sf = _empty(*views[1], dtype=torch.float8_e4m3fn, device=x.device)
+        sf_perm = _empty(*views[2], dtype=torch.float8_e4m3fn, device=x.device)
     h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_NVFP4, packed.data_ptr(), sf_perm=sf_perm.data_ptr(),
              sf=sf.data_ptr())
     return (packed, sf, sf_perm), h

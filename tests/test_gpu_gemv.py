@@ -11,6 +11,9 @@ scale stops):
   the output is rounded once: eps/2 |y|, or half its smallest step.
 """
 import os
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -466,6 +469,36 @@ def test_expert_block_together_and_captured(t, topk):
         want = O.moe_combine(down.cpu().numpy(), np.arange(t * topk, dtype=np.int32), share.cpu().numpy(), t, topk)
         assert np.array_equal(total.cpu().numpy(), want)
     del graph
+
+
+FIRST_CALLS = """
+import sys
+import torch
+from nvfp4_b200 import _lib, gemv, norm
+g = torch.Generator().manual_seed(0)
+b = torch.randint(0, 256, (300, 320), generator=g, dtype=torch.uint8).cuda()
+sf = torch.randint(0x20, 0x40, (3, 10, 32, 4, 4), generator=g, dtype=torch.uint8).cuda()
+w = gemv.Weights(b, sf)
+gain = torch.ones(640, dtype=torch.bfloat16, device="cuda")
+xs = [torch.randn(m, 640, generator=g).bfloat16().cuda() for m in (1, 9)]
+torch.cuda.synchronize()
+s = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.stream(s):
+    with torch.cuda.graph(graph, stream=s):
+        out = [gemv.dual_gemv(norm.rms_norm(x, gain)[0], w, w) for x in xs]
+    graph.replay()
+torch.cuda.synchronize()
+for x, y in zip(xs, out):
+    assert torch.equal(y, gemv.dual_gemv(norm.rms_norm(x, gain)[0], w, w)) and bool(y.any())
+assert _lib.device_status() == 0
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": str(Path(V.__file__).resolve().parents[1])})
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_expert_table_is_not_made_inside_a_capture():
