@@ -25,7 +25,7 @@
 // An infinite or NaN element makes its 16 elements' scale NaN, and with it
 // every output of that token.
 //
-// With few tokens gemv_kernel expands x itself, four warps of each CTA for its
+// With few tokens gemv_kernel expands x itself, eight warps of each CTA for its
 // part of K, while the first weights are on their way.  With more that would
 // be the slowest part (about 300 warp instructions for a token's 256
 // elements), and gemv_expand_kernel does it once, as images of the shared memory that the MMAs
@@ -497,14 +497,14 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSma
 // shared memory: each CTA owns 128 / splits rows, gets the others' sums for them and
 // adds them in the order of the CTAs.
 //
-// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 13.6 us (4.9
+// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 13.2 us (5.0
 // TB/s); a ring of 90 KB without any MMA, all of the GPU reading 66 MB of other data, takes 14.1, plain
 // 32-byte loads 12.4 (10.1 us at the rate of a long copy: what is short here is the time).  The
-// gated pair 14336 x 4096 (66 MB) 14.3 us, 8 experts of a token, gated, 2048 x 7168 (132 MB) 24.6 (the
-// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 59.4 us, 5.9 TB/s.  Smaller calls are bound by the
+// gated pair 14336 x 4096 (66 MB) 13.9 us, 8 experts of a token, gated, 2048 x 7168 (132 MB) 24.0 (the
+// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 57 us, 6.1 TB/s.  Smaller calls are bound by the
 // chain from the end of the work before to the first product and from the last to the output, about
 // 4 us: 4.5 us for 1001 x 1536 (0.9 MB).  More tokens cost the expansion, 0.1 us of epilogue each
-// and room for fewer weights on their way: 7168 x 16384 14.6 us for one, 19.3 for 16.
+// and room for fewer weights on their way: 7168 x 16384 14.3 us for one, 18.8 for 16.
 template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
 __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __grid_constant__ GemvParams p) {
   constexpr int kMats = kDual ? 2 : 1;
@@ -591,7 +591,10 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   if (warp == kWWarp) {
     // ------------------------------------------------------------ weights
     if (elect_one()) {
-      const uint64_t pol = policy_evict_normal();
+      // read once, they leave L2 to what is read again (x's images, the next kernel's input): 3 tokens 14336 x
+      // 4096 10.3 us, 11.2 with the normal policy; 64 rows of experts 7168 x 2048 60.6 and 63.2 (over 3 to
+      // 10 GB of weights).  More groups of the same weights find them in L2.
+      const uint64_t pol = p.passes == 1 ? policy_evict_first() : policy_evict_normal();
       int slot = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
