@@ -1209,14 +1209,13 @@ namespace {
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
-// Device workspace of a call: [groups (experts)][factors][images].
-struct GemvSpace { size_t back, image, total; };
+// Device workspace of a call: [factors][images].
+struct GemvSpace { size_t image, total; };
 
-GemvSpace gemv_space(bool moe, long long rows, long long groups, int k) {
+GemvSpace gemv_space(long long rows, long long groups, int k) {
   const size_t k_blocks = (size_t)((k + kBK - 1) / kBK);
   GemvSpace s;
-  s.back = moe ? align_up(sizeof(GemvGroups), 256) : 0;
-  s.image = align_up(s.back + (size_t)groups * kGemvTokens * kGemvMaxSplits * sizeof(float), 256);
+  s.image = align_up((size_t)groups * kGemvTokens * kGemvMaxSplits * sizeof(float), 256);
   s.total = s.image + k_blocks * ((size_t)rows * kGemvTokenBytes + (size_t)groups * kGemvXSfBytes);
   return s;
 }
@@ -1269,10 +1268,10 @@ int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
 size_t gemv_workspace(int x_dtype, bool x_vec, int m, int n, int k, int l, int num_sms) {
   int splits;
   if (gemv_expands_itself(x_dtype, x_vec, m, gemv_span(m, n, k, l, num_sms, &splits))) return 0;
-  return gemv_space(false, (long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
+  return gemv_space((long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
 }
 size_t moe_gemv_workspace(int x_dtype, bool x_vec, int pairs, int k) {
-  return gemv_expands_itself(x_dtype, x_vec, pairs) ? 0 : gemv_space(true, pairs, pairs, k).total;
+  return gemv_expands_itself(x_dtype, x_vec, pairs) ? 0 : gemv_space(pairs, pairs, k).total;
 }
 
 template <class Kern>
@@ -1342,10 +1341,9 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   p.splits = gemv_splits(tiles, p.k_blocks, d->num_sms, p.group_rows);
   p.split_bits = p.splits == 8 ? 3 : p.splits / 2;
   if (!kMoe) self = gemv_expands_itself(p.x_dtype, p.x_vec, p.m, (p.k_blocks + p.splits - 1) / p.splits);
-  const GemvSpace sp = gemv_space(kMoe, kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
+  const GemvSpace sp = gemv_space(kMoe ? p.pairs : (long long)p.l * p.m, groups, p.k);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
-  p.groups = reinterpret_cast<GemvGroups*>(ws);
-  p.back = reinterpret_cast<float*>(ws + sp.back);
+  p.back = reinterpret_cast<float*>(ws);
   p.image = ws + sp.image;
   p.status = d->status;
   p.wait_limit = wait_limit_cycles();
@@ -1358,7 +1356,7 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   const int send = self ? kGemvSend<true> : kGemvSend<false>;
   const int sums = p.splits > 1 ? kMats * ((p.group_rows + send - 1) / send * send) * kBM * (int)sizeof(float) : 0;
   const bool shared_sm = p.splits == 8 && p.group_rows <= kGemvSelfTokens && tiles > gemv_lone_clusters(d->num_sms);
-  const int budget = (shared_sm ? 112 : 216) * 1024;
+  const int budget = (shared_sm ? 112 : kMoe && !self ? 208 : 216) * 1024;   // experts: a CTA of the expansion fits beside it
   p.x_slots = self ? kGemvMaxXSlots : kMoe || p.group_rows > 8 ? 4 : 6;
   p.w_slots = (budget - 1024 - sums - p.x_slots * x_bytes) / kGemvWBytes;
   if (p.w_slots > kGemvMaxWSlots) p.w_slots = kGemvMaxWSlots;

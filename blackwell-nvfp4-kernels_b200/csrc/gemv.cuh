@@ -36,6 +36,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <cstdint>
+#include <type_traits>
 #include "kernel_common.cuh"
 #include "ptx.cuh"
 #include "quantize.cuh"
@@ -58,13 +59,18 @@ struct alignas(64) GemvExpert {
   const uint8_t* sf;
 };
 
-// Groups of an expert call: an expert and up to 16 of its rows.
+// Groups of an expert call: an expert and up to 16 of its rows.  Both kernels make
+// them for themselves from the ids.
 struct GemvGroups {
   int count;
-  int expert[kGemvMaxPairs];
   int rows[kGemvMaxPairs];
-  int before[kGemvMaxPairs];             // rows in the groups before
-  int pair[kGemvMaxPairs];               // [before + i]: row of x's pairs
+  uint16_t expert[kGemvMaxPairs];
+  uint16_t before[kGemvMaxPairs];        // rows in the groups before
+  uint16_t pair[kGemvMaxPairs];          // [before + i]: row of x's pairs
+};
+struct GemvGroupScratch {
+  uint16_t seen[kGemvMaxExperts], open[kGemvMaxExperts];        // an expert's rows so far, its last group
+  int16_t group_of[kGemvMaxPairs], place_of[kGemvMaxPairs];
 };
 
 struct GemvParams {
@@ -90,7 +96,6 @@ struct GemvParams {
   int pairs, topk, experts;
   int x_per_pair;                        // x has a row for each pair, not for each token
   const GemvExpert *table1, *table2;
-  GemvGroups* groups;
   unsigned* status;
   long long wait_limit;
 };
@@ -280,31 +285,30 @@ __device__ __forceinline__ void gemv_put(float (&v)[8], float up, uint8_t* token
 }
 
 // Pairs of one expert in ascending order, p.room at a time; one warp, the result in shared memory.
-__device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups& out, int* seen, int* open,
-                                                 int* group_of, int* place_of) {
+__device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups& out, GemvGroupScratch& tmp) {
   const int lane = (int)(threadIdx.x & 31u);
   const uint32_t lt = (1u << lane) - 1u;
-  for (int i = lane; i < p.experts; i += 32) seen[i] = 0;
+  for (int i = lane; i < p.experts; i += 32) tmp.seen[i] = 0;
   __syncwarp();
   int groups = 0;
   for (int i0 = 0; i0 < p.pairs; i0 += 32) {
     const int i = i0 + lane;
-    const int id = i < p.pairs ? __ldg(p.ids + i) : -1;
+    const int id = i < p.pairs ? __ldcg(p.ids + i) : -1;
     const bool valid = (unsigned)id < (unsigned)p.experts;
     const uint32_t same = __match_any_sync(0xffffffffu, valid ? id : -1);
-    const int before = valid ? seen[id] : 0, at = before + __popc(same & lt);
-    const int old = valid && before > 0 ? open[id] : 0;
+    const int before = valid ? tmp.seen[id] : 0, at = before + __popc(same & lt);
+    const int old = valid && before > 0 ? tmp.open[id] : 0;
     const bool first = valid && at % p.room == 0;
     const uint32_t firsts = __ballot_sync(0xffffffffu, first);
     int grp = groups + __popc(firsts & lt);
     const uint32_t mine = firsts & same & (lt | (1u << lane));   // the group's first row, if it is among these 32
     const int theirs = __shfl_sync(0xffffffffu, grp, mine ? 31 - __clz(mine) : lane);
     grp = mine ? theirs : old;
-    if (first) out.expert[grp] = id, out.rows[grp] = 0;
+    if (first) out.expert[grp] = (uint16_t)id, out.rows[grp] = 0;
     __syncwarp();
     if (valid) atomicAdd(&out.rows[grp], 1);
-    if (valid && (same >> lane) == 1u) seen[id] = at + 1, open[id] = grp;   // the expert's last row among these
-    if (i < p.pairs) group_of[i] = valid ? grp : -1, place_of[i] = at % p.room;
+    if (valid && (same >> lane) == 1u) tmp.seen[id] = (uint16_t)(at + 1), tmp.open[id] = (uint16_t)grp;   // the expert's last row among these
+    if (i < p.pairs) tmp.group_of[i] = (int16_t)(valid ? grp : -1), tmp.place_of[i] = (int16_t)(at % p.room);
     groups += __popc(firsts);
     __syncwarp();
   }
@@ -317,13 +321,13 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (g0 + lane < groups) out.before[g0 + lane] = sum + x - rows;
+    if (g0 + lane < groups) out.before[g0 + lane] = (uint16_t)(sum + x - rows);
     sum += __shfl_sync(0xffffffffu, x, 31);
   }
   if (lane == 0) out.count = groups;
   __syncwarp();
   for (int i = lane; i < p.pairs; i += 32)
-    if (group_of[i] >= 0) out.pair[out.before[group_of[i]] + place_of[i]] = i;
+    if (tmp.group_of[i] >= 0) out.pair[out.before[tmp.group_of[i]] + tmp.place_of[i]] = (uint16_t)i;
 }
 
 // grid: (row of x, chunk of 8 K blocks, split).  A CTA takes the largest magnitude
@@ -332,9 +336,6 @@ __device__ __forceinline__ void gemv_group_pairs(const GemvParams& p, GemvGroups
 template <bool kMoe>
 __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __grid_constant__ GemvParams p) {
   __shared__ uint32_t s_top[kExpandThreads / 32];
-  __shared__ GemvGroups s_groups;
-  __shared__ int s_seen[kMoe ? kGemvMaxExperts : 1], s_open[kMoe ? kGemvMaxExperts : 1];
-  __shared__ int s_group_of[kMoe ? kGemvMaxPairs : 1], s_place_of[kMoe ? kGemvMaxPairs : 1];
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch_dependents();                            // after the wait: see the head of this file
@@ -342,16 +343,11 @@ __global__ void __launch_bounds__(kExpandThreads) gemv_expand_kernel(const __gri
   int group, place, rows, before, rows_all, groups_all;
   int64_t src;
   if constexpr (kMoe) {
-    if (warp == 0) gemv_group_pairs(p, s_groups, s_seen, s_open, s_group_of, s_place_of);
+    __shared__ GemvGroups s_groups;
+    __shared__ GemvGroupScratch s_tmp;
+    if (warp == 0) gemv_group_pairs(p, s_groups, s_tmp);
     __syncthreads();
-    if (r == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
-      if (tid == 0) p.groups->count = s_groups.count;
-      for (int i = tid; i < p.pairs; i += kExpandThreads) {
-        p.groups->expert[i] = s_groups.expert[i], p.groups->rows[i] = s_groups.rows[i];
-        p.groups->before[i] = s_groups.before[i], p.groups->pair[i] = s_groups.pair[i];
-      }
-    }
-    group = s_group_of[r], place = s_place_of[r];
+    group = s_tmp.group_of[r], place = s_tmp.place_of[r];
     if (group < 0) {                                      // not an expert: a row of zeros
       for (int c = (int)(blockIdx.z * gridDim.y + blockIdx.y) * kExpandThreads + tid; c < p.n; c += (int)(gridDim.y * gridDim.z) * kExpandThreads)
         store_out(p.out, p.out_dtype, (int64_t)r * p.ldo + c, 0.f);
@@ -468,17 +464,17 @@ struct GemvSmallGroups {
   int pair[kGemvSelfPairs][kGemvSelfTokens], x_row[kGemvSelfPairs][kGemvSelfTokens];
 };
 
-template <bool kMoe, bool kSelf>
-__device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSmallGroups& small, int t) {
+__device__ __forceinline__ int gemv_pair(const GemvSmallGroups& g, const GemvTile& t, int row) { return g.pair[t.group][row]; }
+__device__ __forceinline__ int gemv_pair(const GemvGroups& g, const GemvTile& t, int row) { return g.pair[t.before + row]; }
+
+template <bool kMoe, bool kSelf, class Groups>
+__device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const Groups& groups, int t) {
   GemvTile r;
   if constexpr (kMoe) {
     r.group = t / p.row_blocks, r.row_block = t - r.group * p.row_blocks, r.batch = 0;
-    if constexpr (kSelf) {
-      r.expert = small.expert[r.group], r.rows = small.rows[r.group], r.before = 0;
-    } else {
-      r.expert = __ldcg(&p.groups->expert[r.group]);
-      r.rows = __ldcg(&p.groups->rows[r.group]), r.before = __ldcg(&p.groups->before[r.group]);
-    }
+    r.expert = groups.expert[r.group], r.rows = groups.rows[r.group];
+    if constexpr (kSelf) r.before = 0;
+    else r.before = groups.before[r.group];
   } else {
     // groups of the same weights next to one another: they share them in L2 (the branches spare
     // two divisions, about 0.1 us, where they are not needed)
@@ -501,7 +497,7 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const GemvSma
 // TB/s); a ring of 90 KB without any MMA, all of the GPU reading 66 MB of other data, takes 14.1, plain
 // 32-byte loads 12.4 (10.1 us at the rate of a long copy: what is short here is the time).  The
 // gated pair 14336 x 4096 (66 MB) 13.9 us, 8 experts of a token, gated, 2048 x 7168 (132 MB) 24.0 (the
-// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 57 us, 6.1 TB/s.  Smaller calls are bound by the
+// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 55 us, 6.3 TB/s.  Smaller calls are bound by the
 // chain from the end of the work before to the first product and from the last to the output, about
 // 4 us: 4.5 us for 1001 x 1536 (0.9 MB).  More tokens cost the expansion, 0.1 us of epilogue each
 // and room for fewer weights on their way: 7168 x 16384 14.3 us for one, 18.8 for 16.
@@ -520,7 +516,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   // of the tokens of tile index % 2: 2^-e, and the row of out (experts)
   __shared__ float s_back[2][kSelf ? kGemvSelfTokens : kGemvTokens];
   __shared__ int s_row[2][kGemvTokens];
-  __shared__ GemvSmallGroups s_small;
+  __shared__ std::conditional_t<!kMoe, char, std::conditional_t<kSelf, GemvSmallGroups, GemvGroups>> s_groups;
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = (int)threadIdx.x >> 5, lane = (int)(threadIdx.x & 31u);
@@ -555,7 +551,15 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     fence_proxy_async_smem();
   }
   if (warp == kMmaWarp) tmem_alloc<kTmemCols>(smem_u32(&s_tmem_base));
-  if constexpr (kMoe) griddep_wait();                     // the experts' ids, or the groups from the expansion
+  if constexpr (kMoe && !kSelf) {
+    // like the weights the ids are there when the expansion lets this kernel start (64 rows of experts
+    // 7168 x 2048 55.0 us, 57.3 with the expansion's groups); the ring is scratch until its first load
+    if (warp == 0) {
+      gemv_group_pairs(p, s_groups, *reinterpret_cast<GemvGroupScratch*>(smem_raw));
+      fence_proxy_async_smem();
+    }
+  }
+  if constexpr (kMoe && kSelf) griddep_wait();            // the experts' ids
   if constexpr (kMoe && kSelf) {
     // rows of one expert in ascending order, kGemvSelfTokens at a time
     if (warp == 0) {
@@ -570,11 +574,11 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
       const int from = valid ? 31 - __clz(mine) : lane;
       const int grp = __shfl_sync(0xffffffffu, __popc(firsts & lt), from);
       if (valid) {
-        s_small.pair[grp][at % kGemvSelfTokens] = lane;
-        s_small.x_row[grp][at % kGemvSelfTokens] = p.x_per_pair ? lane : lane / p.topk;
+        s_groups.pair[grp][at % kGemvSelfTokens] = lane;
+        s_groups.x_row[grp][at % kGemvSelfTokens] = p.x_per_pair ? lane : lane / p.topk;
       }
-      if (first) s_small.expert[grp] = id, s_small.rows[grp] = min(kGemvSelfTokens, __popc(same) - at);
-      if (lane == 0) s_small.count = __popc(firsts);
+      if (first) s_groups.expert[grp] = id, s_groups.rows[grp] = min(kGemvSelfTokens, __popc(same) - at);
+      if (lane == 0) s_groups.count = __popc(firsts);
     }
   }
   tc_fence_before();
@@ -584,8 +588,9 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   const uint32_t tmem = s_tmem_base;
   const AbortCtl ctl{&s_abort, p.status, p.wait_limit};
   if (threadIdx.x == 0) griddep_launch_dependents();
-  const int tiles = !kMoe ? p.l * p.passes * p.row_blocks
-                          : (kSelf ? s_small.count : __ldcg(&p.groups->count)) * p.row_blocks;
+  int tiles;
+  if constexpr (kMoe) tiles = s_groups.count * p.row_blocks;
+  else tiles = p.l * p.passes * p.row_blocks;
   const int atoms_all = p.k / kKStep;                     // 64-deep atoms of a 128-row block
 
   if (warp == kWWarp) {
@@ -604,7 +609,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
         if (cluster < tiles) ctl.wait(smem_u32(&bar_go), 0, kDevTimeoutStageFree);
       }
       for (int t = cluster; t < tiles && ok; t += clusters) {
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         const void *map[2] = {&p.map1, &p.map2};
         const uint8_t* sf[2] = {p.sf1, p.sf2};
         if constexpr (kMoe) {
@@ -616,7 +621,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           const int atoms = min(kBK / kKStep, atoms_all - kb * (kBK / kKStep));
           #pragma unroll
           for (int mat = 0; mat < kMats; ++mat) {
-            if (!kSelf && !kMoe && slot == 0 && phase == 1u) griddep_wait();   // the ring is full: again, no polling
+            if (!kSelf && slot == 0 && phase == 1u) griddep_wait();   // the ring is full: again, no polling
             if (!ctl.wait(smem_u32(&bar_w_free[slot]), phase ^ 1u, kDevTimeoutStageFree)) {
               ok = false;
               break;
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
       for (int t = cluster; t < tiles && ok; t += clusters) {
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         const uint32_t bytes = tc.rows * kGemvTokenBytes + kGemvXSfBytes;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ctl.wait(smem_u32(&bar_x_free[slot]), phase ^ 1u, kDevTimeoutStageFree)) {
@@ -688,7 +693,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
       uint32_t w_phase = 0, x_phase = 0, acc_phase = 0;
       bool ok = true, any = false;
       for (int t = cluster; t < tiles && ok; t += clusters, done += span) {
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         const int n_cols = (tc.rows * kGemvTerms + 15) / 16 * 16;
         const int xsf_at = (kSelf ? p.group_rows : tc.rows) * kGemvTokenBytes;
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(n_cols >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
@@ -752,9 +757,9 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     auto expand = [&](int t, int index) -> bool {
       bool ok = true;
       if constexpr (kSelf) {                              // x in 16 bits, 16-byte aligned
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         auto x_at = [&](int tok) -> int64_t {
-          if constexpr (kMoe) return (int64_t)s_small.x_row[tc.group][tok] * p.ldx;
+          if constexpr (kMoe) return (int64_t)s_groups.x_row[tc.group][tok] * p.ldx;
           return (int64_t)tc.batch * p.x_batch + (int64_t)(tc.before - tc.batch * p.m + tok) * p.ldx;
         };
         static_assert(kGemvSelfTokens == 2, "token of an item: its last bit");
@@ -833,11 +838,11 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     int acc_buf = 0;
     auto finish = [&](int t, int index) -> bool {
         constexpr int kStep = kGemvStep<kSelf>, kSend = kGemvSend<kSelf>;
-        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_small, t);
+        const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         // before the wait: a load for each token in the loops below is 0.3 us a token
         if (row < tc.rows) {
           if constexpr (!kSelf) s_back[index % 2][row] = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + row) * splits + rank);
-          if constexpr (kMoe) s_row[index % 2][row] = kSelf ? s_small.pair[tc.group][row] : __ldcg(&p.groups->pair[tc.before + row]);
+          if constexpr (kMoe) s_row[index % 2][row] = gemv_pair(s_groups, tc, row);
         }
         bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
         if (splits > 1 && t != cluster)

@@ -350,6 +350,29 @@ def test_moe_gemv_out_rows_apart_and_one_choice_vector():
     assert bool(torch.isnan(big[:, :16]).all()) and bool(torch.isnan(big[:, 112:]).all())
 
 
+@pytest.mark.parametrize("tokens", [3, 12, 50])
+def test_moe_gemv_ids_weights_and_x_written_just_before(tokens):
+    """What the stream's last kernels wrote, the ids and weights too, which the call reads first."""
+    w, _ = make_experts(8, 1024, 2048, seed=1)
+    other, _ = make_experts(8, 1024, 2048, seed=60)
+    g = torch.Generator().manual_seed(tokens)
+    sets = [(torch.randint(-1, 8, (tokens, 4), generator=g, dtype=torch.int32).cuda(),
+             torch.randn(tokens, 2048, generator=g).bfloat16().cuda(), e) for e in (w, other, w)]
+    want = [moe.gemv(x, ids, e) for ids, x, e in sets]
+    live, _ = make_experts(8, 1024, 2048, seed=1)
+    ids, x = sets[0][0].clone(), sets[0][1].clone()
+    torch.cuda.synchronize()
+    for i in range(30):
+        now_ids, now_x, now_w = sets[i % 3]
+        for (b, sf), (nb, ns) in zip(live.w, now_w.w):
+            b.view(torch.uint8).copy_(nb.view(torch.uint8))
+            sf.view(torch.uint8).copy_(ns.view(torch.uint8))
+        x.copy_(now_x)
+        ids.copy_(now_ids)
+        assert torch.equal(moe.gemv(x, ids, live), want[i % 3]), i
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_moe_gemv_unaligned_x_and_strided_choices(dtype):
     w, d = make_experts(6, 160, 448, seed=20)
