@@ -513,8 +513,12 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   __shared__ uint32_t s_tmem_base;
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_top[kGemvSelfTokens];             // expansion: largest magnitudes
-  // of the tokens of tile index % 2: 2^-e, and the row of out (experts)
-  __shared__ float s_back[2][kSelf ? kGemvSelfTokens : kGemvTokens];
+  // Of the tokens of a tile: 2^-e (tile index % kBackSlots), and the row of out (index % 2, experts).  finish(i) reads
+  // both, and its first barrier lies behind all that finish(i - 1) reads: written inside finish(i), two slots do.
+  // expand(i) writes 2^-e before finish(i - 1), when a warp may still be in finish(i - 2) (no barrier of the whole CTA
+  // comes between them where the group stays the same and nothing is exchanged): slots i, i - 1 and i - 2 differ.
+  constexpr int kBackSlots = kSelf ? 4 : 2;
+  __shared__ float s_back[kBackSlots][kSelf ? kGemvSelfTokens : kGemvTokens];
   __shared__ int s_row[2][kGemvTokens];
   __shared__ std::conditional_t<!kMoe, char, std::conditional_t<kSelf, GemvSmallGroups, GemvGroups>> s_groups;
 
@@ -801,7 +805,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           named_bar_sync(2, 256);
           seen = tc.group;
         }
-        if (tid < tc.rows) s_back[index % 2][tid] = exp2_int(-gemv_exponent(s_top[tid]));
+        if (tid < tc.rows) s_back[index % kBackSlots][tid] = exp2_int(-gemv_exponent(s_top[tid]));
         __syncwarp();
         for (int i0 = 0; i0 < items && ok; i0 += 32) {
           if (i0 > 0) load_batch(raw, i0);
@@ -841,7 +845,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
         const GemvTile tc = gemv_tile<kMoe, kSelf>(p, s_groups, t);
         // before the wait: a load for each token in the loops below is 0.3 us a token
         if (row < tc.rows) {
-          if constexpr (!kSelf) s_back[index % 2][row] = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + row) * splits + rank);
+          if constexpr (!kSelf) s_back[index % kBackSlots][row] = __ldcg(p.back + ((int64_t)tc.group * kGemvTokens + row) * splits + rank);
           if constexpr (kMoe) s_row[index % 2][row] = gemv_pair(s_groups, tc, row);
         }
         bool ok = ctl.wait(smem_u32(&bar_acc_full[acc_buf]), acc_phase, kDevTimeoutAccFull);
@@ -880,7 +884,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
             // it 20.0); sums behind the last token's are not stored
             v[0][i] = v[1][i] = 0.f;
             if (!kSelf || t0 + i < tc.rows) {
-              const float back = s_back[index % 2][t0 + i];
+              const float back = s_back[index % kBackSlots][t0 + i];
               #pragma unroll
               for (int a = 0; a < 2; ++a)
                 if (a == 0 || both) {

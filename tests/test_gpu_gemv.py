@@ -405,6 +405,73 @@ def test_moe_gemv_non_finite_tokens_are_nan_and_leave_the_others():
 
 
 # ---------------------------------------------------------------------------
+# many tiles for each CTA
+# ---------------------------------------------------------------------------
+def raw_weights(n, k, seed, l=1):
+    """(packed [l, n, k/2], atoms [l, rows/128, k/64, 32, 4, 4], dense fp64 [l, n, k]) on the GPU, of random
+    codes and scales: large ones quickly."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    rb = -(-n // 128)
+    packed = torch.randint(0, 256, (l, n, k // 2), generator=g, dtype=torch.uint8, device="cuda")
+    atoms = torch.randint(0x20, 0x40, (l, rb, k // 64, 32, 4, 4), generator=g, dtype=torch.uint8, device="cuda")
+    table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64, device="cuda")
+    codes = torch.stack((packed & 15, packed >> 4), -1).reshape(l, n, k // 16, 16)
+    # [l, row block, quarter, row of 32, atom, block of 16]
+    scales = atoms.view(torch.float8_e4m3fn).double().permute(0, 1, 4, 3, 2, 5).reshape(l, rb * 128, k // 16)[:, :n]
+    return packed, atoms, (table[codes.int()] * scales.unsqueeze(-1)).reshape(l, n, k)
+
+
+def products_there(x, w):
+    """:func:`products` on the GPU, for large weights."""
+    x = x.double()
+    m, k = x.shape
+    a = torch.maximum(x.abs().reshape(m, k // 16, 16).amax(2), 2.0 ** -14 * x.abs().amax(1, keepdim=True))
+    bound = a.repeat_interleave(16, 1) @ w.abs().T * (2.0 ** -22 + (k / 64 + 16) * 2.0 ** -23 * 16 / 7)
+    return (x @ w.T).cpu().numpy(), bound.cpu().numpy()
+
+
+def scaled_rows(rows, k, seed, dtype=torch.bfloat16):
+    """Rows whose magnitudes differ by powers of two: a sum taken back with another row's factor shows."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(rows, k, generator=g, device="cuda")
+    return (x * torch.exp2(((torch.arange(rows, device="cuda") * 5) % 7 - 3).float())[:, None]).to(dtype)
+
+
+@pytest.mark.parametrize("l,m,n,k", [(2, 1, 20480, 2048), (2, 2, 20480, 512), (3, 1, 20000, 320), (7, 2, 3000, 512)])
+def test_gemv_batch_entries_that_share_a_ctas_tiles(l, m, n, k):
+    """A CTA's tiles go over from one batch entry to the next: each row gets its own factor."""
+    packed, atoms, dense = raw_weights(n, k, seed=n + l, l=l)
+    w = V.Weights(packed.permute(1, 2, 0), atoms)
+    x = scaled_rows(l * m, k, seed=k).view(l, m, k)
+    first = V.gemv(x, w, out_dtype=torch.float32)
+    for b in range(l):
+        check(first[b], *products_there(x[b], dense[b]))
+        gated = V.dual_gemv(x, w, w, out_dtype=torch.float32)
+        y, e = products_there(x[b], dense[b])
+        with np.errstate(over="ignore"):
+            check(gated[b], *gate(y, e, y, e))
+    for _ in range(20):
+        assert torch.equal(V.gemv(x, w, out_dtype=torch.float32), first)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [3, 16])
+def test_moe_gemv_choices_that_share_a_ctas_tiles(rows):
+    """The same with one expert's tiles after another's."""
+    e, n, k = 3, 19200, 256
+    packed, atoms, dense = raw_weights(n, k, seed=rows, l=e)
+    w = moe.ExpertWeights(list(zip(packed, atoms)))
+    x = scaled_rows(rows, k, seed=rows, dtype=torch.float16)
+    ids = (torch.arange(rows, dtype=torch.int32, device="cuda") * 2) % e
+    first = moe.gemv(x, ids, w, out_dtype=torch.float32)
+    for p, ex in enumerate(ids.tolist()):
+        check(first[p:p + 1], *products_there(x[p:p + 1], dense[ex]))
+    for _ in range(20):
+        assert torch.equal(moe.gemv(x, ids, w, out_dtype=torch.float32), first)
+    assert _lib.device_status() == 0
+
+
+# ---------------------------------------------------------------------------
 # a run of the operators together, captured and replayed
 # ---------------------------------------------------------------------------
 def _capture(fn):
