@@ -113,6 +113,13 @@ __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");
 }
 
+// Before the first use of a tensor map that lies in global memory: makes what was written there (by a
+// copy or a kernel before this one) visible to the copies that this thread issues, whose descriptors may
+// otherwise come from a cache that still holds those of an earlier map at the same address.
+__device__ __forceinline__ void tensor_map_acquire(const void* map) {
+  asm volatile("fence.proxy.tensormap::generic.acquire.sys [%0], 128;" ::"l"(map) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar,
                                             int c0, int c1, int c2, uint64_t policy) {
   asm volatile(

@@ -471,6 +471,28 @@ def test_moe_gemv_choices_that_share_a_ctas_tiles(rows):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("tokens", [2, 12])
+def test_moe_gemv_table_rewritten_in_place(tokens):
+    """Another table at the same address: its descriptors count, not the ones that a call before has read.
+    All weights stay alive."""
+    sets = [make_experts(6, 640, 1024, seed=s)[0] for s in (1, 30, 60)]
+    x = torch.randn(tokens, 1024, generator=torch.Generator().manual_seed(tokens)).bfloat16().cuda()
+    ids = (torch.arange(tokens * 4, dtype=torch.int32, device="cuda") % 6).view(tokens, 4)
+    want = [(moe.gemv(x, ids, w), moe.dual_gemv(x, ids, w, w)) for w in sets]
+    live = make_experts(6, 640, 1024, seed=1)[0]
+    for i in range(60):
+        live.table().copy_(sets[i % 3].table())
+        assert torch.equal(moe.gemv(x, ids, live), want[i % 3][0]), i
+        assert torch.equal(moe.dual_gemv(x, ids, live, live), want[i % 3][1]), i
+    at = set()
+    for i in range(6):                                     # and a new object's table where a dropped one's was
+        fresh = moe.ExpertWeights(sets[i % 3].w)
+        at.add(fresh.table().data_ptr())
+        assert torch.equal(moe.gemv(x, ids, fresh), want[i % 3][0]), i
+        del fresh
+    assert len(at) < 6 and _lib.device_status() == 0
+
+
 # ---------------------------------------------------------------------------
 # a run of the operators together, captured and replayed
 # ---------------------------------------------------------------------------
