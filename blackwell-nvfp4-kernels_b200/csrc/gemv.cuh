@@ -128,9 +128,11 @@ constexpr int kExpandBlocks = kExpandThreads / 32;        // K blocks of a CTA
 
 // Eight consecutive elements as they lie in memory (b: fp32 only).  kVec: 16-byte aligned.
 struct Raw8 { uint4 a, b; };
-__device__ __forceinline__ uint4 ldg_v4(const void* q) {   // volatile: stays in front of a signal that follows it
+// From L2, and not by the path of read-only data (ld.global.nc): a kernel of this file starts while the one before
+// it may still write x and the ids.  Volatile: the load stays in front of a signal that follows it.
+__device__ __forceinline__ uint4 ldcg_v4(const void* q) {
   uint4 v;
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(q));
+  asm volatile("ld.global.cg.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(q));
   return v;
 }
 template <bool kWide, bool kVec>
@@ -140,19 +142,19 @@ __device__ __forceinline__ Raw8 gemv_raw8(const void* x, int64_t at) {
   if constexpr (kWide) {
     const uint32_t* q = static_cast<const uint32_t*>(x) + at;
     if constexpr (kVec) {
-      r.a = ldg_v4(q), r.b = ldg_v4(q + 4);
+      r.a = ldcg_v4(q), r.b = ldcg_v4(q + 4);
     } else {
-      r.a = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
-      r.b = make_uint4(__ldg(q + 4), __ldg(q + 5), __ldg(q + 6), __ldg(q + 7));
+      r.a = make_uint4(__ldcg(q), __ldcg(q + 1), __ldcg(q + 2), __ldcg(q + 3));
+      r.b = make_uint4(__ldcg(q + 4), __ldcg(q + 5), __ldcg(q + 6), __ldcg(q + 7));
     }
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(x) + at;
     if constexpr (kVec) {
-      r.a = ldg_v4(q);
+      r.a = ldcg_v4(q);
     } else {
       uint32_t v[4];
       #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
+      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__ldcg(q + 2 * i) | (uint32_t)__ldcg(q + 2 * i + 1) << 16;
       r.a = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     // rows of one expert in ascending order, kGemvSelfTokens at a time
     if (warp == 0) {
       const uint32_t lt = (1u << lane) - 1u;
-      const int id = lane < p.pairs ? __ldg(p.ids + lane) : -1;
+      const int id = lane < p.pairs ? __ldcg(p.ids + lane) : -1;
       const bool valid = (unsigned)id < (unsigned)p.experts;
       const uint32_t same = __match_any_sync(0xffffffffu, valid ? id : -1);
       const int at = __popc(same & lt);
@@ -764,7 +766,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
     const int own_bits = kBMBits - p.split_bits, own_rows = 1 << own_bits, owner = row >> own_bits;   // the CTA that finishes this thread's row
     if constexpr (kMoe && kSelf) {                        // rows without an expert are zero
       for (int i = (int)blockIdx.x; i < p.pairs; i += (int)gridDim.x)
-        if ((unsigned)__ldg(p.ids + i) >= (unsigned)p.experts)
+        if ((unsigned)__ldcg(p.ids + i) >= (unsigned)p.experts)
           for (int c = row; c < p.n; c += 256) store_out(p.out, p.out_dtype, (int64_t)i * p.ldo + c, 0.f);
     }
     // Expansion of a tile's x.  A warp takes one token's K block at a time, a lane
@@ -791,7 +793,7 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
           for (int u = 0; u < 4; ++u) {
             const int i = i0 + 8 * u + me, k0 = (kb0 + (i >> two)) * kBK + lane * 8;
             r[u] = make_uint4(0, 0, 0, 0);
-            if (i < items && k0 < p.k) r[u] = ldg_v4(static_cast<const uint16_t*>(p.x) + x_at(i & two) + k0);
+            if (i < items && k0 < p.k) r[u] = ldcg_v4(static_cast<const uint16_t*>(p.x) + x_at(i & two) + k0);
           }
         };
         uint4 raw[4];

@@ -231,6 +231,49 @@ def test_gemv_on_two_streams_at_once():
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("m,n", [(1, 2048), (2, 2048), (5, 2048), (1, 192)])
+def test_gemv_to_and_fro_between_two_buffers(m, n):
+    """A chain of calls that each overwrite what the call before read, and that may start before it ends: as with
+    a pause after each."""
+    g = torch.Generator("cuda").manual_seed(n)
+    b = torch.randint(0, 256, (n, n // 2), generator=g, dtype=torch.uint8, device="cuda")
+    # codes of mean square 8.6 at scale 2^-7 (2^-5 for 192): a step's growth is about 1
+    sf = torch.full((-(-n // 128), n // 64, 32, 4, 4), 0x04 if n == 2048 else 0x10, dtype=torch.uint8, device="cuda")
+    w = V.Weights(b, sf)
+    start = torch.randn(m, n, generator=g, device="cuda").bfloat16()
+
+    def chain(pause):
+        bufs = [start.clone(), torch.empty_like(start)]
+        torch.cuda.synchronize()
+        seen = []
+        for i in range(40):
+            V.gemv(bufs[i % 2], w, out=bufs[1 - i % 2])
+            if pause:
+                torch.cuda.synchronize()
+            if i % 10 == 9:
+                seen.append(bufs[1 - i % 2].clone())
+        return seen
+
+    want = chain(True)
+    assert all(bool(torch.isfinite(t).all()) and bool(t.any()) for t in want)
+    for _ in range(10):
+        for a, c in zip(chain(False), want):
+            assert torch.equal(a, c)
+    graph, out = _capture(lambda: chain_captured(w, start))
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[-1])
+    del graph
+
+
+def chain_captured(w, start):
+    bufs = [start.clone(), torch.empty_like(start)]
+    for i in range(40):
+        V.gemv(bufs[i % 2], w, out=bufs[1 - i % 2])
+    return bufs[0]
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_gemv_on_another_device():
     w, dense = make_weights(200, 512, seed=4)
