@@ -198,7 +198,10 @@ def combine(c_all: torch.Tensor, d: Dispatch, weights: torch.Tensor | None = Non
     ``weights`` fp32 [T] or [T, topk], None for all ones."""
     if c_all.dim() != 2 or c_all.dtype != torch.float16 or not c_all.is_contiguous():
         raise ValueError("c_all must be a contiguous float16 tensor [rows, N]")
-    n = c_all.shape[1]
+    n, dst = c_all.shape[1], d.dst
+    if (dst.device != c_all.device or dst.dtype != torch.int32 or dst.numel() != d.tokens * d.topk
+            or not dst.is_contiguous()):
+        raise ValueError(f"the order of {d.tokens} x {d.topk} rows must be contiguous int32 on c_all's device")
     if weights is not None:
         weights = weights.reshape(d.tokens, d.topk)
         if weights.dtype != torch.float32 or weights.device != c_all.device:
@@ -206,11 +209,14 @@ def combine(c_all: torch.Tensor, d: Dispatch, weights: torch.Tensor | None = Non
         weights = weights.contiguous()
     if out is None:
         out = torch.empty((d.tokens, n), dtype=torch.float32, device=c_all.device)
-    elif tuple(out.shape) != (d.tokens, n) or out.dtype != torch.float32 or not out.is_contiguous():
-        raise ValueError("out must be a contiguous float32 tensor [tokens, N]")
+    elif (tuple(out.shape) != (d.tokens, n) or out.dtype != torch.float32 or not out.is_contiguous()
+          or out.device != c_all.device):
+        raise ValueError("out must be a contiguous float32 tensor [tokens, N] on c_all's device")
+    if not c_all.is_cuda:
+        raise ValueError("c_all must be a CUDA tensor")
     lib = _lib.load()
     _lib.check(on_device(c_all.device, lambda st: lib.nvfp4_moe_combine(
-        c_all.data_ptr(), c_all.shape[0], d.dst.data_ptr(),
+        c_all.data_ptr(), c_all.shape[0], dst.data_ptr(),
         weights.data_ptr() if weights is not None else None,
         d.tokens, d.topk, n, out.data_ptr(), st)))
     return out

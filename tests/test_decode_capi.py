@@ -121,3 +121,18 @@ def test_digits_of_x_stay_within_their_bound():
     assert digits.min() >= -4 and digits.max() <= 3
     back = sum(d / 2 * 8.0 ** -j for j, d in enumerate(digits))
     assert np.abs(back - x).max() <= 2.0 ** -23
+
+
+def test_combine_refuses_an_order_out_or_rows_on_the_host():
+    """Addresses of host memory never reach a kernel."""
+    rows = torch.zeros(6, 64, dtype=torch.float16, device="meta")     # stands for another device
+    with pytest.raises(ValueError, match="CUDA"):
+        moe.combine(torch.zeros(6, 64, dtype=torch.float16), moe.pair_order(3, 2, "cpu"))
+    with pytest.raises(ValueError, match="order"):
+        moe.combine(rows, moe.pair_order(3, 2, "cpu"))
+    for dst in (torch.zeros(6, dtype=torch.int64, device="meta"), torch.zeros(5, dtype=torch.int32, device="meta"),
+                torch.zeros(12, dtype=torch.int32, device="meta")[::2]):
+        with pytest.raises(ValueError, match="order"):
+            moe.combine(rows, moe.PairOrder(dst, 3, 2))
+    with pytest.raises(ValueError, match="out"):
+        moe.combine(rows, moe.pair_order(3, 2, "meta"), out=torch.zeros(3, 64))
