@@ -25,6 +25,21 @@ DTYPES = {torch.float32: _lib.NVFP4_F32, torch.float16: _lib.NVFP4_F16,
           torch.bfloat16: _lib.NVFP4_BF16}
 
 
+def check_scales(name: str, t: torch.Tensor, n: int, k: int, l: int, device) -> None:
+    """``t`` must be the permuted scales of L matrices [N, K] or their memory (see :class:`Weights`)."""
+    atoms = (ceil_div(n, 128), k // 64, 32, 4, 4)
+    shape = tuple(t.shape)
+    if shape == (l,) + atoms or (l == 1 and shape == atoms):
+        if t.dtype not in (torch.float8_e4m3fn, torch.uint8, torch.int8):
+            raise ValueError(f"{name}: expected float8_e4m3fn, got {t.dtype}")
+        if not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name} must be contiguous on {device}")
+    elif t.dim() == 6 and shape[:2] == (32, 4):
+        check_sf_perm(name, t, n, k, l, device)
+    else:
+        raise ValueError(f"{name}: shape {shape} holds no scales of [{n}, {k}, {l}]")
+
+
 class Weights:
     """One NVFP4 weight matrix (or L of them), checked once.
 
@@ -45,16 +60,7 @@ class Weights:
             raise ValueError(f"b: N={n}, L={l} must be positive and K={k} a positive multiple of 64")
         if b.stride(1) != 1 or (n > 1 and b.stride(0) != kh) or (l > 1 and b.stride(2) != n * kh):
             raise ValueError(f"b: strides {b.stride()} are not the K-major [L][{n}][{kh}] layout")
-        if sfb_perm.dim() == 6 and tuple(sfb_perm.shape[:2]) == (32, 4):
-            check_sf_perm("sfb_perm", sfb_perm, n, k, l, b.device)
-        else:
-            atoms = (ceil_div(n, 128), k // 64, 32, 4, 4)
-            if tuple(sfb_perm.shape) not in ((l,) + atoms, *((atoms,) if l == 1 else ())):
-                raise ValueError(f"sfb_perm: shape {tuple(sfb_perm.shape)} holds no scales of [{n}, {k}, {l}]")
-            if sfb_perm.dtype not in (torch.float8_e4m3fn, torch.uint8, torch.int8):
-                raise ValueError(f"sfb_perm: expected float8_e4m3fn, got {sfb_perm.dtype}")
-            if not sfb_perm.is_contiguous() or sfb_perm.device != b.device:
-                raise ValueError(f"sfb_perm must be contiguous on {b.device}")
+        check_scales("sfb_perm", sfb_perm, n, k, l, b.device)
         self.b, self.sfb_perm = b, sfb_perm
         self.n, self.k, self.l, self.device = n, k, l, b.device
         self.ptrs = (b.data_ptr(), sfb_perm.data_ptr())

@@ -136,3 +136,19 @@ def test_combine_refuses_an_order_out_or_rows_on_the_host():
             moe.combine(rows, moe.PairOrder(dst, 3, 2))
     with pytest.raises(ValueError, match="out"):
         moe.combine(rows, moe.pair_order(3, 2, "meta"), out=torch.zeros(3, 64))
+
+
+def test_scales_of_32_matrices_of_four_row_blocks_are_their_memory():
+    """[32, 4, K/64, 32, 4, 4], contiguous, is the memory of 32 matrices and not the permuted view of one."""
+    t = torch.zeros(32, 4, 2, 32, 4, 4, dtype=torch.uint8)
+    gemv.check_scales("sf", t, 512, 128, 32, t.device)
+    gemv.check_scales("sf", t.view(torch.float8_e4m3fn), 400, 128, 32, t.device)
+    view = t.permute(3, 4, 1, 5, 2, 0)                       # the permuted view of the same
+    gemv.check_scales("sf", view, 512, 128, 32, t.device)
+    one = torch.zeros(4, 2, 32, 4, 4, dtype=torch.uint8)
+    gemv.check_scales("sf", one, 512, 128, 1, t.device)
+    for bad, n, k, l in ((t, 512, 128, 31), (t, 640, 128, 32), (t, 512, 192, 32), (view.contiguous(), 512, 128, 32),
+                         (t.float(), 512, 128, 32), (one, 512, 128, 2), (one.transpose(0, 1), 256, 256, 1),
+                         (t.to("meta"), 512, 128, 32)):
+        with pytest.raises(ValueError):
+            gemv.check_scales("sf", bad, n, k, l, t.device)

@@ -274,6 +274,16 @@ def chain_captured(w, start):
     return bufs[0]
 
 
+def test_gemv_of_32_matrices_of_four_row_blocks():
+    """Their scales' memory has the permuted view's first two extents."""
+    packed, atoms, dense = raw_weights(500, 128, seed=3, l=32)
+    x = torch.randn(32, 1, 128, generator=torch.Generator("cuda").manual_seed(1), device="cuda").bfloat16()
+    y = V.gemv(x, V.Weights(packed.permute(1, 2, 0), atoms))
+    assert torch.equal(y, V.gemv(x, V.Weights(packed.permute(1, 2, 0), atoms.permute(3, 4, 1, 5, 2, 0))))
+    for b in range(32):
+        check(y[b], *products_there(x[b], dense[b]))
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_gemv_on_another_device():
     w, dense = make_weights(200, 512, seed=4)
