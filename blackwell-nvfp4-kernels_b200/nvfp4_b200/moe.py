@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .dual_gemm import on_device
+from .dual_gemm import check_sf_perm, on_device
 from .gemv import DTYPES, _empty, _launch, _rows_last
 
 
@@ -129,10 +129,28 @@ def grouped_inputs(d: Dispatch, weights, c_all: torch.Tensor, counts=None):
     return (abc, sfab, sfab_perm, sizes), which
 
 
+BYTES = (torch.uint8, torch.int8)
+
+
+def _check_expert_scales(name, t, n, k, device):
+    """One expert's permuted scales or their memory in any contiguous shape, but not plain [N, K/16] ones, which
+    hold as many bytes where N is a multiple of 128."""
+    rn, rk = -(-n // 128), k // 64
+    if t.numel() != rn * rk * 512 or t.device != device:
+        raise ValueError(f"{name} must hold {rn * rk * 512} bytes on {device}")
+    if t.dtype not in BYTES + (torch.float8_e4m3fn,):
+        raise ValueError(f"{name}: expected float8_e4m3fn, got {t.dtype}")
+    view = t.unsqueeze(-1) if t.dim() == 5 else t
+    if tuple(view.shape) == (32, 4, rn, 4, rk, 1):
+        check_sf_perm(name, view, n, k, 1, device)
+    elif not t.is_contiguous() or tuple(t.shape) in ((n, k // 16), (n, k // 16, 1), (1, n, k // 16)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, strides {t.stride()} are not the permuted layout of [{n}, {k}]")
+
+
 class ExpertWeights:
     """Per-expert NVFP4 weights for :func:`grouped_gemm`: ``w[e]`` = (b [N, K/2, 1]
-    float4_e2m1fn_x2 (or uint8 [N, K/2]), sfb_perm [32, 4, ceil(N/128), 4, K/64, 1]),
-    all on one device.  The pointer arrays for the C call are built once."""
+    float4_e2m1fn_x2 (or uint8 [N, K/2]), sfb_perm [32, 4, ceil(N/128), 4, K/64, 1] or its
+    memory), all on one device.  The pointer arrays for the C call are built once."""
 
     def __init__(self, w):
         self.w = list(w)
@@ -146,9 +164,9 @@ class ExpertWeights:
                 raise ValueError(f"expert {i}: weights must be CUDA [{self.n}, {self.k // 2}(, 1)]")
             if b.stride(0) != self.k // 2 or b.stride(1) != 1 or b.device != b0.device:
                 raise ValueError(f"expert {i}: weights must be row-major [N][K/2] on {b0.device}")
-            rn, rk = -(-self.n // 128), self.k // 64
-            if sfb.numel() != rn * rk * 512 or sfb.device != b0.device:
-                raise ValueError(f"expert {i}: scales must hold {rn * rk * 512} bytes on {b0.device}")
+            if b.dtype not in BYTES + (torch.float4_e2m1fn_x2,):
+                raise ValueError(f"expert {i}: expected float4_e2m1fn_x2 weights, got {b.dtype}")
+            _check_expert_scales(f"expert {i}: scales", sfb, self.n, self.k, b0.device)
         self.b_ptrs = arr(*[b.data_ptr() for b, _ in self.w])
         self.sfb_ptrs = arr(*[s.data_ptr() for _, s in self.w])
         self.device = b0.device

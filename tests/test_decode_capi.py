@@ -152,3 +152,18 @@ def test_scales_of_32_matrices_of_four_row_blocks_are_their_memory():
                          (t.to("meta"), 512, 128, 32)):
         with pytest.raises(ValueError):
             gemv.check_scales("sf", bad, n, k, l, t.device)
+
+
+def test_experts_scales_are_checked_for_type_and_layout():
+    n, k = 256, 128
+    memory = torch.zeros(2, 2, 32, 4, 4, dtype=torch.uint8)
+    view = memory.view(1, 2, 2, 32, 4, 4).permute(3, 4, 1, 5, 2, 0)
+    dev = memory.device
+    for good in (memory, memory.view(-1), memory.view(1, 2, 2, 32, 4, 4), memory.view(torch.float8_e4m3fn), view, view[..., 0],
+                 memory.view(4, 512), memory.view(torch.int8)):
+        moe._check_expert_scales("sf", good, n, k, dev)
+    plain = torch.zeros(n, k // 16, dtype=torch.uint8)       # as many bytes, in another order
+    for bad in (plain, plain.unsqueeze(-1), plain.view(torch.float8_e4m3fn), plain[None], view.contiguous(), memory.float(),
+                memory.half(), memory.transpose(0, 1), memory[:1], memory.to("meta")):
+        with pytest.raises(ValueError):
+            moe._check_expert_scales("sf", bad, n, k, dev)

@@ -717,3 +717,12 @@ def test_moe_gemv_refuses():
         moe.dual_gemv(x, ids, w, other)
     with pytest.raises(_lib.Nvfp4Error, match="at most 256"):
         moe.gemv(torch.zeros(129, 128, device="cuda").half(), torch.zeros(129, 2, dtype=torch.int32, device="cuda"), w)
+
+
+def test_expert_weights_refuse_other_types_and_plain_scales():
+    packed, atoms, _ = raw_weights(128, 128, seed=1)
+    b, sf = packed[0], atoms[0]
+    moe.ExpertWeights([(b, sf), (b.view(torch.float4_e2m1fn_x2).unsqueeze(-1), sf.view(-1))])
+    for bad in ((b.half(), sf), (b, sf.float()), (b, sf.reshape(128, 8)), (b, sf.reshape(128, 8, 1))):
+        with pytest.raises(ValueError):
+            moe.ExpertWeights([(b, sf), bad])
