@@ -197,6 +197,8 @@ def grouped_gemm(d: Dispatch, weights: ExpertWeights, c_all: torch.Tensor) -> to
     if len(weights) != d.experts or weights.k != d.k:
         raise ValueError(f"weights are for {len(weights)} experts x K={weights.k}, "
                          f"dispatch has {d.experts} x K={d.k}")
+    if weights.device != d.packed.device:
+        raise ValueError(f"weights are on {weights.device}, the dispatch on {d.packed.device}")
     rows = d.tokens * d.topk
     if (c_all.dtype != torch.float16 or tuple(c_all.shape) != (rows, weights.n)
             or not c_all.is_contiguous() or c_all.device != d.packed.device):

@@ -167,3 +167,16 @@ def test_experts_scales_are_checked_for_type_and_layout():
                 memory.half(), memory.transpose(0, 1), memory[:1], memory.to("meta")):
         with pytest.raises(ValueError):
             moe._check_expert_scales("sf", bad, n, k, dev)
+
+
+def test_grouped_gemm_refuses_weights_on_another_device():
+    class Elsewhere:
+        n, k, device = 128, 64, torch.device("cpu")
+
+        def __len__(self):
+            return 2
+
+    i32 = torch.zeros(3, dtype=torch.int32, device="meta")
+    d = moe.Dispatch(torch.zeros(4, 32, dtype=torch.uint8, device="meta"), i32, i32, i32, i32, i32, i32, i32, 4, 1, 64, 2)
+    with pytest.raises(ValueError, match="weights are on"):
+        moe.grouped_gemm(d, Elsewhere(), torch.zeros(4, 128, dtype=torch.float16, device="meta"))
