@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1213,7 +1214,7 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 struct GemvSpace { size_t image, total; };
 
 GemvSpace gemv_space(long long rows, long long groups, int k) {
-  const size_t k_blocks = (size_t)((k + kBK - 1) / kBK);
+  const size_t k_blocks = (size_t)((k - 1) / kBK + 1);
   GemvSpace s;
   s.image = align_up((size_t)groups * kGemvTokens * kGemvMaxSplits * sizeof(float), 256);
   s.total = s.image + k_blocks * ((size_t)rows * kGemvTokenBytes + (size_t)groups * kGemvXSfBytes);
@@ -1259,8 +1260,8 @@ bool gemv_expands_itself(int x_dtype, bool x_vec, int pairs) { return x_dtype !=
 
 // K blocks of a CTA.
 int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
-  const int k_blocks = (k + kBK - 1) / kBK;
-  const long long tiles = (long long)l * ((m + kGemvTokens - 1) / kGemvTokens) * ((n + kBM - 1) / kBM);
+  const int k_blocks = (k - 1) / kBK + 1;
+  const long long tiles = (long long)l * ((m - 1) / kGemvTokens + 1) * ((n - 1) / kBM + 1);
   *splits = gemv_splits(tiles, k_blocks, num_sms, m < kGemvTokens ? m : kGemvTokens);
   return (k_blocks + *splits - 1) / *splits;
 }
@@ -1268,7 +1269,7 @@ int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
 size_t gemv_workspace(int x_dtype, bool x_vec, int m, int n, int k, int l, int num_sms) {
   int splits;
   if (gemv_expands_itself(x_dtype, x_vec, m, gemv_span(m, n, k, l, num_sms, &splits))) return 0;
-  return gemv_space((long long)l * m, (long long)l * ((m + kGemvTokens - 1) / kGemvTokens), k).total;
+  return gemv_space((long long)l * m, (long long)l * ((m - 1) / kGemvTokens + 1), k).total;
 }
 size_t moe_gemv_workspace(int x_dtype, bool x_vec, int pairs, int k) {
   return gemv_expands_itself(x_dtype, x_vec, pairs) ? 0 : gemv_space(pairs, pairs, k).total;
@@ -1327,7 +1328,7 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   t_pdl = kn.pdl;
   constexpr int kMats = kDual ? 2 : 1;
   p.k_blocks = (p.k + kBK - 1) / kBK;
-  p.row_blocks = (p.n + kBM - 1) / kBM;
+  p.row_blocks = (p.n - 1) / kBM + 1;
   p.passes = (p.m + kGemvTokens - 1) / kGemvTokens;
   const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
   const long long tiles = (long long)groups * p.row_blocks;
@@ -1384,6 +1385,7 @@ bool dtype_ok(int t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
 // Sizes, types and alignment that all the products share.
 constexpr int kGemvMaxRows = 4096;       // rows of x in a batch entry
 constexpr int kGemvMaxK = 1 << 20;
+constexpr int kGemvMaxN = INT_MAX - (1 << 21);   // columns are counted in 32 bits, in steps of up to 2^20 (zero rows)
 
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (bytes < need || (need > 0 && !workspace))
@@ -1397,6 +1399,7 @@ int validate_gemv(const GemvParams& p) {
   if (!dtype_ok(p.x_dtype) || !dtype_ok(p.out_dtype)) return fail(NVFP4_ERR_INVALID_ARG, "bad dtype (x %d, out %d)", p.x_dtype, p.out_dtype);
   if (p.k % 64 != 0) return fail(NVFP4_ERR_SHAPE, "K=%d is not a multiple of 64", p.k);
   if (p.k > kGemvMaxK) return fail(NVFP4_ERR_SHAPE, "K=%d (at most %d)", p.k, kGemvMaxK);
+  if (p.n > kGemvMaxN) return fail(NVFP4_ERR_SHAPE, "N=%d (at most %d)", p.n, kGemvMaxN);
   // kernels count tiles (row blocks of every 16 rows of x, or of every choice) and x's elements in 32 bits
   const long long groups = p.pairs ? p.pairs : (long long)p.l * ((p.m + kGemvTokens - 1) / kGemvTokens);
   if (groups * (p.n / kBM + 1LL) >= (1LL << 30) || (long long)p.m * p.l * p.k >= (1LL << 31))

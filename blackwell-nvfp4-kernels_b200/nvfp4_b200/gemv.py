@@ -93,6 +93,8 @@ def _run(x, w, w2, out, out_dtype):
     if shape[-1] != k or (shape[0] if dims == 3 else 1) != l:
         raise ValueError(f"x {tuple(shape)} does not match weights of K={k}, L={l}")
     m = shape[-2]
+    if m >> 31:
+        raise ValueError(f"{m} rows: at most 4096 of a matrix")
     x = _rows_last(x)
     want = (l, m, n) if dims == 3 else (m, n)
     if out is None:

@@ -255,6 +255,8 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
     rows, n, k = tokens * topk, w.n, w.k
     if x.shape[1] != k or x.shape[0] not in (tokens, rows):
         raise ValueError(f"x {tuple(x.shape)} is neither [{tokens}, {k}] nor [{rows}, {k}]")
+    if rows >> 31:
+        raise ValueError(f"{rows} rows: at most 256")
     x, ids = _rows_last(x), ids.contiguous()
     if out is None:
         out = _empty((rows, n), (n, 1), dtype=out_dtype or x.dtype, device=x.device)

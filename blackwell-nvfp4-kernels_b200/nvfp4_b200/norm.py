@@ -36,6 +36,8 @@ def _check(x, weight, residual, residual_out):
         raise ValueError(f"weight must be float16, bfloat16 or float32 [{k}] on {device}")
     if k < 1:
         raise ValueError("K must be positive")
+    if rows >> 31:
+        raise ValueError(f"{rows} rows: at most 2^31 - 1")
     x = _rows_last(x)
     if weight.stride(0) != 1:
         weight = weight.contiguous()

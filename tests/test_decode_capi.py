@@ -180,3 +180,11 @@ def test_grouped_gemm_refuses_weights_on_another_device():
     d = moe.Dispatch(torch.zeros(4, 32, dtype=torch.uint8, device="meta"), i32, i32, i32, i32, i32, i32, i32, 4, 1, 64, 2)
     with pytest.raises(ValueError, match="weights are on"):
         moe.grouped_gemm(d, Elsewhere(), torch.zeros(4, 128, dtype=torch.float16, device="meta"))
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 128, 2 ** 31 - 2 ** 20])
+def test_widths_next_to_32_bits_are_refused(lib, n):
+    """The kernels count columns in 32 bits, in steps of up to 2^20."""
+    assert _gemv(lib, n=n, ldo=n, k=64, ldx=64) == SHAPE
+    one = ctypes.c_void_p(4096)
+    assert lib.nvfp4_moe_gemv(one, F16, 64, 0, one, 1, 1, one, None, 8, one, F16, n, n, 64, one, 1 << 30, None) == SHAPE

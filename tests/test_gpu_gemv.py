@@ -726,3 +726,19 @@ def test_expert_weights_refuse_other_types_and_plain_scales():
     for bad in ((b.half(), sf), (b, sf.float()), (b, sf.reshape(128, 8)), (b, sf.reshape(128, 8, 1))):
         with pytest.raises(ValueError):
             moe.ExpertWeights([(b, sf), bad])
+
+
+def test_rows_past_32_bits_are_refused():
+    """Counts of rows that a C int would cut off."""
+    from nvfp4_b200 import norm
+    packed, atoms, _ = raw_weights(1, 64, seed=1)
+    many = torch.zeros(1, 64, device="cuda").half().expand(2 ** 32 + 1, 64)
+    with pytest.raises(ValueError, match="rows"):
+        V.gemv(many, V.Weights(packed[0], atoms[0]))
+    ids = torch.zeros(1, 1, dtype=torch.int32, device="cuda").expand(2 ** 32 + 1, 1)
+    with pytest.raises(ValueError, match="rows"):
+        moe.gemv(many, ids, moe.ExpertWeights([(packed[0], atoms[0])]))
+    gain = torch.ones(64, device="cuda")
+    for f in (norm.rms_norm, norm.rms_norm_fp8, norm.rms_norm_nvfp4):
+        with pytest.raises(ValueError, match="rows"):
+            f(many, gain, **({"group": None} if f is norm.rms_norm_fp8 else {}))
