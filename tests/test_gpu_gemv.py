@@ -524,6 +524,53 @@ def test_moe_gemv_choices_that_share_a_ctas_tiles(rows):
     assert _lib.device_status() == 0
 
 
+# (batch entries, rows, N, K): more row blocks than a GPU has SMs, so that a CTA takes several tiles; the last two with the K
+# of a tile shared between CTAs
+WIDE = [(1, 1, 20000, 1024), (1, 2, 20000, 2048), (1, 1, 128256, 1024), (1, 2, 128256, 512), (3, 1, 20000, 704),
+        (20, 2, 2300, 2304), (1, 5, 20000, 512), (1, 1, 25600, 8192), (2, 1, 12800, 8192)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("l,m,n,k", WIDE)
+def test_gemv_several_tiles_a_cta(l, m, n, k, dtype):
+    packed, atoms, dense = raw_weights(n, k, seed=n + k, l=l)
+    w = V.Weights(packed.permute(1, 2, 0), atoms)
+    x = scaled_rows(l * m, k, seed=m, dtype=TYPES[dtype]).view(l, m, k)
+    one, two = V.gemv(x, w, out_dtype=torch.float32), V.dual_gemv(x, w, w, out_dtype=torch.float32)
+    for b in range(l):
+        y, e = products_there(x[b], dense[b])
+        check(one[b], y, e)
+        with np.errstate(over="ignore"):
+            check(two[b], *gate(y, e, y, e))
+    del dense
+    torch.cuda.empty_cache()
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("tokens,topk,e,n,k", [(1, 8, 8, 7168, 2048), (4, 8, 10, 7168, 2048), (16, 2, 8, 7168, 512), (32, 1, 1, 2048, 1024),
+                                               (1, 8, 8, 3200, 8192), (5, 8, 8, 7168, 512)])
+def test_moe_gemv_several_tiles_a_cta(tokens, topk, e, n, k):
+    """One token's experts, and choices that repeat an expert up to 32 times."""
+    packed, atoms, dense = raw_weights(n, k, seed=tokens + n, l=e)
+    w = moe.ExpertWeights(list(zip(packed, atoms)))
+    g = torch.Generator().manual_seed(tokens)
+    ids = torch.randint(0, e, (tokens, topk), generator=g, dtype=torch.int32) if tokens > 1 else torch.randperm(e, generator=g)[None, :topk].int()
+    for rows in {tokens, tokens * topk}:
+        x = scaled_rows(rows, k, seed=rows)
+        one = moe.gemv(x, ids.cuda(), w, out_dtype=torch.float32)
+        two = moe.dual_gemv(x, ids.cuda(), w, w, out_dtype=torch.float32)
+        per = x if rows == tokens * topk else x.repeat_interleave(topk, 0)
+        for ex in set(ids.reshape(-1).tolist()):
+            at = (ids.reshape(-1) == ex).nonzero()[:, 0].cuda()
+            y, err = products_there(per[at], dense[ex])
+            check(one[at], y, err)
+            with np.errstate(over="ignore"):
+                check(two[at], *gate(y, err, y, err))
+    del dense
+    torch.cuda.empty_cache()
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("tokens", [2, 12])
 def test_moe_gemv_table_rewritten_in_place(tokens):
     """Another table at the same address: its descriptors count, not the ones that a call before has read.
