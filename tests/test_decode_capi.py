@@ -188,3 +188,22 @@ def test_widths_next_to_32_bits_are_refused(lib, n):
     assert _gemv(lib, n=n, ldo=n, k=64, ldx=64) == SHAPE
     one = ctypes.c_void_p(4096)
     assert lib.nvfp4_moe_gemv(one, F16, 64, 0, one, 1, 1, one, None, 8, one, F16, n, n, 64, one, 1 << 30, None) == SHAPE
+
+
+def test_bound_of_one_elements_digits_tells_seven_digits_from_eight():
+    """The bound that the GPU test of single elements uses, on the host: kept by eight digits, broken without the last."""
+    import numpy as np
+    rng = np.random.default_rng(1)
+    x = (rng.standard_normal(4000) * 2.0 ** rng.integers(-12, 12, 4000)).astype(np.float32).astype(np.float64)
+    s = 2.0 ** np.ceil(np.log2(np.abs(x) / 1.5))
+    fields = np.rint(x / s * 2.0 ** 22).astype(np.int64) + 0x924924
+    digits = [(((fields >> (3 * (7 - j))) & 7) - 4) / 2 for j in range(8)]
+    bound = np.abs(x) * (8 / 3 + 3.5) * 2.0 ** -24
+
+    def joined(n):
+        v = np.zeros(len(x), np.float32)
+        for d in reversed(digits[:n]):
+            v = (v.astype(np.float64) / 8 + d).astype(np.float32)     # one rounding, as fmaf
+        return v * s
+    assert (np.abs(joined(8) - x) <= bound).all()
+    assert (np.abs(joined(7) - x) > bound).mean() > 0.2
