@@ -602,10 +602,12 @@ __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __gr
   if (warp == kWWarp) {
     // ------------------------------------------------------------ weights
     if (elect_one()) {
-      // read once, they leave L2 to what is read again (x's images, the next kernel's input): 3 tokens 14336 x
-      // 4096 10.3 us, 11.2 with the normal policy; 64 rows of experts 7168 x 2048 60.6 and 63.2 (over 3 to
-      // 10 GB of weights).  More groups of the same weights find them in L2.
-      const uint64_t pol = p.passes == 1 ? policy_evict_first() : policy_evict_normal();
+      // Weights that are read once leave L2 to what is read again (x's images, the next kernel's input): 3 tokens 14336 x
+      // 4096 10.3 us, 11.2 with the normal policy.  More groups of one matrix find it in L2.  An expert's groups
+      // are too far apart for that: evict-first is better for any number of tokens, the normal policy hardly ever (64 rows of
+      // experts 7168 x 2048 60.6 and 63.2; 256 rows of 64 experts 2048 x 4096 63.0 and 68.9, all of 8 experts 37.0 and 38.3;
+      // 32 of 8 experts 4096 x 14336 102.7 and 107.5; 256 of 8 experts 7168 x 2048 49.0 and 48.8).
+      const uint64_t pol = kMoe || p.passes == 1 ? policy_evict_first() : policy_evict_normal();
       int slot = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       // The tables are in global memory, where the caller may have written others since the last call.  A tile's maps are
