@@ -1251,12 +1251,21 @@ int gemv_splits(long long tiles, int k_blocks, int num_sms, int group_rows) {
 // Whether gemv_kernel expands x itself: one launch less, but its eight warps
 // take about 1 us for 8 K blocks of a token.  Measured, us with / without: one token 512 x
 // 1024 4.2 / 5.2, 4096 x 14336 (14 K blocks a CTA) 9.8 / 11.2, 16384 x 7168 (28) 13.6 / 15.3; two tokens 8192 x
-// 8192 (32) 10.6 / 12.1, 16384 x 7168 (56) 16.4 / 15.6; four tokens 14336 x 4096 (64) 21 / 12.  8 experts
-// of a token, gated, 2048 x 7168 24.6 / 29.7; 2 experts of a token 4096 x 1536 6.4 / 9.5.
+// 8192 (32) 10.6 / 12.1, 16384 x 7168 (56) 16.4 / 15.6; four tokens 14336 x 4096 (64) 21 / 12.
 bool gemv_expands_itself(int x_dtype, bool x_vec, int rows, int span) {
   return x_dtype != kDtF32 && x_vec && rows <= kGemvSelfTokens && rows * span <= 32;
 }
 bool gemv_expands_itself(int x_dtype, bool x_vec, int pairs) { return x_dtype != kDtF32 && x_vec && pairs <= kGemvSelfPairs; }
+// Whether that form, whose groups have two rows, is also the faster one for experts: where no expert has more rows than that
+// (up to two tokens, which choose different experts) or few have, and where weights read again cost less than the expansion's
+// launch.  Measured, us with / without, tokens x choices of experts: 1 x 8 of 64 7168 x 2048 16.6 / 18.1, gated 2048 x 7168
+// 24.6 / 29.7; 2 x 8 of 64 7168 x 2048 25.2 / 26.0; 4 x 8 of 64 gated 2048 x 7168 72.2 / 75.8; 8 x 4 of 32 gated 2048 x 7168 60.2 / 61.5, 7168 x
+// 2048 38.0 / 31.9; 8 x 1 of 8 4096 x 1536 9.6 / 10.8.  More choices than experts: 16 x 2 of 8 gated 7168 x 4096 83.6 / 49.7, 4096 x 14336
+// 102.6 / 53.4; 4 x 8 of 16 7168 x 2048 35.2 / 25.6; 32 x 1 of 8, all on one, 31.8 / 15.6; 16 x 2 of 8 2048 x 1024 (2^26) 9.3 / 8.9; 8 x 4 of
+// 8 1024 x 1024 6.3 / 7.8; but 6 x 2 of 8 gated 4096 x 4096 25.5 / 28.3.
+bool gemv_few_repeats(int tokens, int pairs, int experts, int n, int k) {
+  return tokens <= kGemvSelfTokens || pairs <= experts || (long long)pairs * n * k <= 1LL << 26;
+}
 
 // K blocks of a CTA.
 int gemv_span(int m, int n, int k, int l, int num_sms, int* splits) {
@@ -1322,8 +1331,9 @@ int launch_gemv(DeviceState* d, int slot, const GemvParams& p, int smem, long lo
                         "gemv_kernel");
 }
 
+// inside: whether gemv_kernel expands x itself (experts; else by gemv_expands_itself)
 template <bool kDual, bool kMoe>
-int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream) {
+int run_gemv(DeviceState* d, GemvParams& p, void* workspace, bool inside, cudaStream_t stream) {
   const Knobs kn = read_knobs();
   t_pdl = kn.pdl;
   constexpr int kMats = kDual ? 2 : 1;
@@ -1333,7 +1343,7 @@ int run_gemv(DeviceState* d, GemvParams& p, void* workspace, cudaStream_t stream
   const int rows = kMoe ? p.pairs : p.m, groups = kMoe ? p.pairs : p.l * p.passes;
   const long long tiles = (long long)groups * p.row_blocks;
   p.room = kGemvTokens;
-  bool self = kMoe && gemv_expands_itself(p.x_dtype, p.x_vec, p.pairs);
+  bool self = kMoe && inside;
   // experts: twice the average of an expert's rows, so that the x slots are not sized for what hardly ever comes
   if (self) p.room = kGemvSelfTokens;
   else if (kMoe)
@@ -1447,7 +1457,7 @@ extern "C" int nvfp4_gemv(const void* x, int x_dtype, long long ldx, long long x
   if ((rc = encode_operand(&p.map1, b1, n, k, l, kBM))) return rc;
   if (b2 && (rc = encode_operand(&p.map2, b2, n, k, l, kBM))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return b2 ? run_gemv<true, false>(d, p, workspace, stream) : run_gemv<false, false>(d, p, workspace, stream);
+  return b2 ? run_gemv<true, false>(d, p, workspace, false, stream) : run_gemv<false, false>(d, p, workspace, false, stream);
 }
 
 extern "C" size_t nvfp4_moe_table_bytes(int num_experts) {
@@ -1509,7 +1519,11 @@ extern "C" int nvfp4_moe_gemv(const void* x, int x_dtype, long long ldx, int x_p
   DeviceState* d = nullptr;
   if ((rc = get_device(&d))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return table2 ? run_gemv<true, true>(d, p, workspace, stream) : run_gemv<false, true>(d, p, workspace, stream);
+  // a workspace that is not needed is used where the expansion before the product pays
+  const bool room = workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                    workspace_bytes >= moe_gemv_workspace(x_dtype, false, p.pairs, k);
+  const bool inside = gemv_expands_itself(x_dtype, p.x_vec, p.pairs) && (!room || gemv_few_repeats(tokens, p.pairs, num_experts, n, k));
+  return table2 ? run_gemv<true, true>(d, p, workspace, inside, stream) : run_gemv<false, true>(d, p, workspace, inside, stream);
 }
 
 // ---------------------------------------------------------------------------

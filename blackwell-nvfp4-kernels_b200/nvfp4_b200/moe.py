@@ -273,8 +273,10 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
     aligned = not (px | ldx * x.element_size()) & 15
     size = w.space.get((tokens, topk, code, aligned))
     if size is None:
-        size = w.space[(tokens, topk, code, aligned)] = lib.nvfp4_moe_gemv_workspace_bytes(code, aligned, tokens,
-                                                                                          topk, k)
+        # three and more tokens that choose more often than there are experts: with the space that an x without alignment
+        # needs, the library takes the form that reads an expert less often where that is faster
+        size = w.space[(tokens, topk, code, aligned)] = lib.nvfp4_moe_gemv_workspace_bytes(
+            code, aligned and (tokens <= 2 or rows <= len(w)), tokens, topk, k)
     space = _empty((size,), (1,), dtype=torch.uint8, device=x.device) if size else None
     _launch(lib.nvfp4_moe_gemv, x.device, (
         px, code, ldx, x.shape[0] == rows and topk > 1, ids.data_ptr(), tokens, topk, w.table().data_ptr(),
@@ -287,7 +289,9 @@ def gemv(x: torch.Tensor, expert_ids: torch.Tensor, weights: ExpertWeights,
          out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Row t*topk + j of the result is x_row . W_eᵀ with e = expert_ids[t, j] (int32
     [T] or [T, topk]): a decoding step's experts without a dispatch, activations not
-    quantised, each chosen expert's weights read once for every 16 of its rows.
+    quantised, each chosen expert's weights read once for every group of its rows (two rows
+    up to 32 in all, unless three and more tokens choose more often than there are experts; else
+    4 to 16 rows, about twice an expert's average).
     ``x``: float16, bfloat16 or float32, [T, K] (token t's row for all its choices)
     or [T*topk, K] (a row for each choice).  A row whose id is outside
     [0, experts) is zero.  Result [T*topk, N] in ``out_dtype`` (x's type by

@@ -176,8 +176,12 @@ size_t nvfp4_gemv_workspace_bytes(int x_dtype, int x_aligned, int m, int n, int 
 /* The same with each row's own expert: out row r = t*topk + j is x_row . B_eᵀ (or
  * gated, table2 not NULL) with e = expert_ids[r] and x_row = x row t, or x row r when
  * x_per_pair is not 0.  Rows whose id is outside [0, num_experts) are zero.  Each
- * expert's weights are read once for every 16 of its rows.  tokens*topk <= 256,
- * num_experts <= 1024.  table1 / table2: device copies (64-byte aligned) of the
+ * expert's weights are read once for every group of its rows: two rows where the
+ * kernel expands x itself (16-byte aligned fp16 or bf16, up to 32 rows in all); else a
+ * power of two from 4 to 16, at least twice an expert's average rows up to that.  tokens*topk <=
+ * 256, num_experts <= 1024.  Up to 32 rows need no workspace if x is aligned; with the bytes
+ * that nvfp4_moe_gemv_workspace_bytes() gives for an x that is not, calls of three and more
+ * tokens whose choices outnumber the experts take the larger groups where that is faster.  table1 / table2: device copies (64-byte aligned) of the
  * nvfp4_moe_table_bytes() bytes that nvfp4_moe_table() writes to host memory for
  * the experts' weights b[e] [N][K/2] and permuted scales sfb_perm[e]; they hold
  * as long as those addresses do.  Counterpart in the reference: the grouped

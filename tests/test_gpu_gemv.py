@@ -571,6 +571,38 @@ def test_moe_gemv_several_tiles_a_cta(tokens, topk, e, n, k):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("tokens,topk,e,n,k,before", [(16, 2, 8, 4096, 1024, True), (4, 8, 16, 4096, 768, True), (16, 2, 8, 512, 1024, False),
+                                                       (2, 8, 4, 14336, 1024, False), (8, 1, 8, 14336, 1024, False)])
+def test_moe_gemv_repeated_experts_with_and_without_space(tokens, topk, e, n, k, before):
+    """A call whose choices repeat the experts expands x before the product, where it has the space for that; either
+    way the products are right."""
+    packed, atoms, dense = raw_weights(n, k, seed=n, l=e)
+    w = moe.ExpertWeights(list(zip(packed, atoms)))
+    ids = torch.randint(0, e, (tokens, topk), generator=torch.Generator().manual_seed(n), dtype=torch.int32).cuda()
+    x = scaled_rows(tokens, k, seed=tokens)
+    lib, rows = _lib.load(), tokens * topk
+    results = []
+    for space in (None, lib.nvfp4_moe_gemv_workspace_bytes(_lib.NVFP4_BF16, 0, tokens, topk, k), "python"):
+        out = torch.full((rows, n), float("nan"), device="cuda")
+        count = lib.nvfp4_launch_count()
+        if space == "python":
+            moe.gemv(x, ids, w, out=out)
+        else:
+            ws = torch.empty(space, dtype=torch.uint8, device="cuda") if space else None
+            _lib.check(lib.nvfp4_moe_gemv(x.data_ptr(), _lib.NVFP4_BF16, k, 0, ids.data_ptr(), tokens, topk, w.table().data_ptr(), None, e,
+                                          out.data_ptr(), _lib.NVFP4_F32, n, n, k, ws.data_ptr() if space else None, space or 0,
+                                          torch.cuda.current_stream().cuda_stream))
+        assert lib.nvfp4_launch_count() - count == (2 if before and space else 1)
+        results.append(out)
+        torch.cuda.synchronize()
+    each = x.double().repeat_interleave(topk, 0)
+    for ex in set(ids.reshape(-1).tolist()):
+        at = ids.reshape(-1) == ex
+        for out in results:
+            check(out[at], *products_there(each[at], dense[ex]))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("tokens", [2, 12])
 def test_moe_gemv_table_rewritten_in_place(tokens):
     """Another table at the same address: its descriptors count, not the ones that a call before has read.
