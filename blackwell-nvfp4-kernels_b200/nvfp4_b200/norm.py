@@ -67,7 +67,6 @@ def _run(x, weight, residual, h, eps, fmt, y, y_dtype=0, ldy=0, scales=None, gro
     _launch(_lib.load().nvfp4_rms_norm, x.device, (
         x.data_ptr(), DTYPES[x.dtype], x.stride(0), *res, weight.data_ptr(), DTYPES[weight.dtype], eps, rows, k,
         fmt, y, y_dtype, ldy, scales, group, sf_perm, sf))
-    return x if residual is None else h
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -77,6 +76,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     default).  x, weight, residual and y may each be float16, bfloat16 or float32;
     ``residual_out`` may be ``residual`` itself and ``out`` may be ``x`` (then updated
     in place); nothing else may overlap."""
+    given = x
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if out is None:
@@ -87,9 +87,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
           or out.dtype != (out_dtype or out.dtype) or (out.stride(1) != 1 and k > 1)
           or (rows > 1 and out.stride(0) < k)):
         raise ValueError(f"out must be [{rows}, {k}], float16, bfloat16 or float32, rows apart, on {x.device}")
-    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_PLAIN, out.data_ptr(), DTYPES[out.dtype],
-             max(out.stride(0), k))
-    return out, h
+    _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_PLAIN, out.data_ptr(), DTYPES[out.dtype],
+         max(out.stride(0), k))
+    return out, given if h is None else h
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -100,6 +100,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     dividing K; None: the row), q = e4m3(y / scale) to nearest even, zeros under a
     zero scale; a NaN gives its group a NaN scale.  ``out``: the (q, scales) of an
     earlier call of the same sizes, reused."""
+    given = x
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if group not in (None, 32, 64, 128):
@@ -116,9 +117,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
                 or q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32
                 or any(t.device != x.device or not t.is_contiguous() for t in out)):
             raise ValueError("out does not match: pass the (q, scales) an earlier call returned")
-    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_FP8, q.data_ptr(), scales=scales.data_ptr(),
-             group=group or 0)
-    return (q, scales), h
+    _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_FP8, q.data_ptr(), scales=scales.data_ptr(),
+         group=group or 0)
+    return (q, scales), given if h is None else h
 
 
 def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -127,6 +128,7 @@ def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
     quantise it, bit for bit, and in the same three tensors (K % 64 == 0);
     a NaN gives its 16 columns a NaN scale.  ``out``: the three tensors of an earlier
     call of the same sizes, reused."""
+    given = x
     x, weight, residual, h = _check(x, weight, residual, residual_out)
     rows, k = x.shape
     if k % 64:
@@ -146,6 +148,6 @@ def rms_norm_nvfp4(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
         packed = _empty(*views[0], dtype=torch.float4_e2m1fn_x2, device=x.device)
         sf = _empty(*views[1], dtype=torch.float8_e4m3fn, device=x.device)
         sf_perm = _empty(*views[2], dtype=torch.float8_e4m3fn, device=x.device)
-    h = _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_NVFP4, packed.data_ptr(), sf_perm=sf_perm.data_ptr(),
-             sf=sf.data_ptr())
-    return (packed, sf, sf_perm), h
+    _run(x, weight, residual, h, eps, _lib.NVFP4_NORM_NVFP4, packed.data_ptr(), sf_perm=sf_perm.data_ptr(),
+         sf=sf.data_ptr())
+    return (packed, sf, sf_perm), given if h is None else h

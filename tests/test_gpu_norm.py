@@ -259,3 +259,15 @@ def test_rms_norm_no_rows_and_refusals():
         norm.rms_norm(x, w, eps=-1.0)
     with pytest.raises(_lib.Nvfp4Error, match="32768"):
         norm.rms_norm(torch.zeros(1, 32776, device="cuda"), torch.zeros(32776, device="cuda"))
+
+
+def test_rms_norm_without_a_residual_returns_x_itself():
+    """Also where the kernel reads a copy of it: what is returned is the stream that the next block adds to."""
+    w = torch.ones(96, device="cuda")
+    for x in (torch.randn(5, 96, device="cuda"), torch.randn(96, 5, device="cuda").T, torch.randn(5, 192, device="cuda")[:, ::2]):
+        want = norm.rms_norm(x.contiguous(), w)[0]
+        y, h = norm.rms_norm(x, w)
+        assert h is x and torch.equal(y, want)
+        assert norm.rms_norm_fp8(x, w, group=32)[1] is x
+    x = torch.randn(64, 5, device="cuda").T
+    assert norm.rms_norm_nvfp4(x, w[:64])[1] is x
