@@ -1,7 +1,7 @@
 // A few tokens times NVFP4 weights on the tensor cores, sm_100a:
 // y = x . Wᵀ, the SiLU-gated pair silu(x . W1ᵀ) * (x . W2ᵀ), and both with the
-// weights of each token's chosen experts.  x is fp16, bf16 or fp32 and loses
-// nothing that an fp32 sum keeps; sums are fp32.
+// weights of each token's chosen experts.  x is fp16, bf16 or fp32, held to 24 bits under the
+// largest of 16 neighbours; sums are fp32.
 //
 // Mathematics.  The block-scaled MMA (tcgen05.mma kind::mxf4nvf4) multiplies
 // e2m1 by e2m1, so x is written as eight balanced base-8 digits.  For 16
@@ -12,6 +12,12 @@
 // they are e2m1 values, and |error| <= s / 4 / 8^7 = 2^-23 s < 2^-22 a.  s is an
 // e4m3 scale (of all eight digits; 2^-6 <= s <= 2^8 after x is multiplied by a
 // power of two 2^e chosen for the token and K range), and the MMA's products are exact.
+// So x is a fixed-point number under its block's largest, and under 2^-14 of the K range's largest: the error
+// is below 2^-22 of the one or 2^-36 of the other.  Against 64 bits a result with weights everywhere is off by
+// as much as an fp32 sum or less.  But where a block's largest element meets a zero code, what its neighbours lose to it
+// is not hidden by its product: one element of 1e4 among 7168 normal ones makes the rows whose weight there is
+// zero off by 1.3e-5 (bf16) to 2.6e-5 (fp32) relative, an fp32 sum's by about 1e-6 or less.  (Eight digits are all that N = 128 columns have room for
+// with 16 tokens.)
 // The digits are eight rows of the MMA's B operand, the weights are its A
 // operand (128 rows), read by the tensor core as they are stored:
 //   D[row][8 token + j] = sum over k of W[row][k] s q_(j+1),
@@ -495,13 +501,14 @@ __device__ __forceinline__ GemvTile gemv_tile(const GemvParams& p, const Groups&
 // shared memory: each CTA owns 128 / splits rows, gets the others' sums for them and
 // adds them in the order of the CTAs.
 //
-// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 13.2 us (5.0
-// TB/s); a ring of 90 KB without any MMA, all of the GPU reading 66 MB of other data, takes 14.1, plain
-// 32-byte loads 12.4 (10.1 us at the rate of a long copy: what is short here is the time).  The
+// Bound: the weights' way from HBM.  One token 16384 x 7168 (66 MB) takes 13.4 us (4.9
+// TB/s); a ring of eight such slots alone, one CTA on each SM copying 66 MB and computing nothing, takes 13.2, plain
+// 32-byte loads 12.3 (10.1 us at the rate of a long copy: what is short here is the time).  The
 // gated pair 14336 x 4096 (66 MB) 13.9 us, 8 experts of a token, gated, 2048 x 7168 (132 MB) 24.0 (the
-// ring 23.8), 64 rows of experts 7168 x 2048 (348 MB) 55 us, 6.3 TB/s.  Smaller calls are bound by the
+// ring 22.7), 64 rows of experts 7168 x 2048 (348 MB) 55 us (the ring 53.5), one token 128256 x 4096 (296 MB) 45.8 us,
+// 6.5 TB/s.  Smaller calls are bound by the
 // chain from the end of the work before to the first product and from the last to the output, about
-// 4 us: 4.5 us for 1001 x 1536 (0.9 MB).  More tokens cost the expansion, 0.1 us of epilogue each
+// 4 us: 4.4 us for 1001 x 1536 (0.9 MB).  More tokens cost the expansion, 0.1 us of epilogue each
 // and room for fewer weights on their way: 7168 x 16384 14.3 us for one, 18.8 for 16.
 template <bool kDual, bool kMoe, bool kSelf, int kTmemCols>
 __global__ void __launch_bounds__(gemv_threads(kSelf), 2) gemv_kernel(const __grid_constant__ GemvParams p) {

@@ -223,13 +223,13 @@ __device__ __forceinline__ void norm_divide(float (&v)[8], float s, bool fast) {
 // and K % 8 == 0.
 //
 // Bound: 7 bytes an element at 16 bits (fp8), 63 us of 8192 x 7168 at the rate of a copy; the
-// kernel takes 66.4 (6.2 TB/s), its instructions (28 an element) 72 % of the issue slots.  16-bit
+// kernel takes 66.2 (6.2 TB/s), its instructions (28 an element) 67 % of the issue slots.  16-bit
 // additions and fp32 products go two at a time (83 us before); the group's columns are a power of
 // two and no register is indexed (75 us with integer divisions, 80 with values in local memory).
 // h stays in registers in its own type, half the registers of fp32 for the 16-bit
 // types: several CTAs fit on an SM, whose loads and arithmetic overlap.
 // Four CTAs of 512 threads on an SM with the types known (32 registers): 8192 x
-// 7168 bf16 to fp8 66.4 us; with three, and the codes by division, 74.0, four 67.7.
+// 7168 bf16 to fp8 66.2 us; with three, and the codes by division, 74.0, four 67.7.
 template <int NV, int kThreads, int kOut, bool kVec, int kType>
 __global__ void __launch_bounds__(kThreads, kThreads == 512 && kType != kNormAnyType ? 4 : 1) norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ double s_sum[32];

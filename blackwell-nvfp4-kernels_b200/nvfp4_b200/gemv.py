@@ -3,7 +3,8 @@
 The GEMMs of this package quantise the activations and work on 128-row tiles.
 For the one to sixteen tokens of a decoding step these products read the same
 weights in the same layout (``quantize.quantize``, ``formats``) once, and take the
-activations as they are, fp16, bf16 or fp32, with fp32 sums:
+activations as they are, fp16, bf16 or fp32, with fp32 sums (each element to 2^-22 of
+the largest of its 16 neighbours, see :func:`gemv`):
 
     w1, w2 = gemv.Weights(b1, sfb1_perm), gemv.Weights(b2, sfb2_perm)
     h = gemv.dual_gemv(x, w1, w2)        # silu(x . W1ᵀ) * (x . W2ᵀ)
@@ -129,9 +130,12 @@ def gemv(x: torch.Tensor, w: Weights, out: torch.Tensor | None = None,
          out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """x . Wᵀ for x [M, K] (or [L, M, K], L matrices): [M, N] (or [L, M, N]) in
     ``out_dtype`` (x's type by default; fp16, bf16 or fp32), one rounding of an
-    fp32 sum.  ``out``: written and returned instead of a new tensor; its rows may
-    be strided; it must not overlap x or the weights.  Meant for M <= 16; every 16 further tokens (8 in fp32) read the
-    weights again."""
+    fp32 sum.  x enters the sums with an error below 2^-22 of the largest of its 16
+    consecutive elements (or of 2^-14 of its row's largest, if that is more): no more than
+    fp32 sums lose, but for outputs whose weights are zero where x is largest.
+    ``out``: written and returned instead of a new tensor; its rows may
+    be strided; it must not overlap x or the weights.  Meant for M <= 16; every 16
+    further tokens read the weights again (M <= 4096, and L * M * K < 2^31)."""
     return _run(x, w, None, out, out_dtype)
 
 

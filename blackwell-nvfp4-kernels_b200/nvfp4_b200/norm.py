@@ -98,7 +98,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     """((q, scales), h): q float8_e4m3fn [rows, K] and scales float32 [rows, K/group]
     with y = q * scale; scale = amax/448 over ``group`` columns (32, 64 or 128,
     dividing K; None: the row), q = e4m3(y / scale) to nearest even, zeros under a
-    zero scale; a NaN gives its group a NaN scale.  ``out``: the (q, scales) of an
+    zero scale; a NaN gives its group a NaN scale.  The quotient is formed from
+    h * weight, without the rounding of the root, in two roundings: a code on a border may
+    differ from the one that the rounded y and scale give.  ``out``: the (q, scales) of an
     earlier call of the same sizes, reused."""
     given = x
     x, weight, residual, h = _check(x, weight, residual, residual_out)

@@ -161,8 +161,8 @@ int nvfp4_moe_combine(const void* c, int c_rows, const int* dst, const float* we
  * ldo >= n elements apart, batch entries out_batch; overlapping neither x nor the
  * weights) is rounded once.  x_dtype and out_dtype are NVFP4_F32, _F16 or _BF16.
  * Weights and permuted scale atoms as for the GEMMs, K % 64 == 0, any N.  An infinity or
- * NaN in x makes that row of out NaN.  m <= 4096, l <= 4096, k <= 2^20; meant for
- * m <= 16, every 16 further rows read the weights again.  `workspace`
+ * NaN in x makes that row of out NaN.  m <= 4096, l <= 4096, k <= 2^20, l * m * k < 2^31,
+ * n <= 2^31 - 2^21; meant for m <= 16, every 16 further rows read the weights again.  `workspace`
  * (nvfp4_gemv_workspace_bytes() on the same device, may be 0; 256-byte aligned) is
  * scratch owned by the call until it completes on `stream`; x_aligned: x and its row and
  * batch strides are multiples of 16 bytes.  No reference counterpart: the reference's
@@ -175,12 +175,12 @@ size_t nvfp4_gemv_workspace_bytes(int x_dtype, int x_aligned, int m, int n, int 
 
 /* The same with each row's own expert: out row r = t*topk + j is x_row . B_eᵀ (or
  * gated, table2 not NULL) with e = expert_ids[r] and x_row = x row t, or x row r when
- * x_per_pair is not 0.  Rows whose id is outside [0, num_experts) are zero.  Each
- * expert's weights are read once for every group of its rows: two rows where the
- * kernel expands x itself (16-byte aligned fp16 or bf16, up to 32 rows in all); else a
- * power of two from 4 to 16, at least twice an expert's average rows up to that.  tokens*topk <=
- * 256, num_experts <= 1024.  Up to 32 rows need no workspace if x is aligned; with the bytes
- * that nvfp4_moe_gemv_workspace_bytes() gives for an x that is not, calls of three and more
+ * x_per_pair is not 0.  Rows whose id is outside [0, num_experts) are zero.  An
+ * expert's weights are read once for every group of its rows.  Groups have two rows where the
+ * kernel expands x itself (16-byte aligned fp16 or bf16, up to 32 rows in all), else 4, 8 or
+ * 16: at least twice an expert's average, as far as 16 goes.  tokens*topk <= 256,
+ * num_experts <= 1024.  Up to 32 aligned rows need no workspace; given as much as
+ * nvfp4_moe_gemv_workspace_bytes() asks for without alignment, calls of three and more
  * tokens whose choices outnumber the experts take the larger groups where that is faster.  table1 / table2: device copies (64-byte aligned) of the
  * nvfp4_moe_table_bytes() bytes that nvfp4_moe_table() writes to host memory for
  * the experts' weights b[e] [N][K/2] and permuted scales sfb_perm[e]; they hold
@@ -204,8 +204,10 @@ size_t nvfp4_moe_table_bytes(int num_experts);
 /* h = x + residual (rounded to the residual's type; h = x when residual is NULL),
  * y = h / sqrt(mean(h^2) + eps) * weight over the K columns of each row, in one
  * pass.  h may be the residual itself and a PLAIN y may be x (the same type and stride);
- * nothing else overlaps.  The sum of squares and the root are fp64, h * r and the product
- * with the weight are rounded to fp32 one after the other.
+ * nothing else overlaps.  The sum of squares and the root are fp64, its reciprocal r is
+ * rounded to fp32, h * r and the product with the weight are rounded to fp32 one after the other.
+ * (r is an fp32 number: it overflows for rows whose mean square plus eps is below 2^-256, and has
+ * fewer bits for those above 2^252.)
  *   PLAIN  y in y_dtype
  *   FP8    scale = amax/448 over `group` columns (32, 64 or 128, dividing K; 0: the
  *          row), y = e4m3_rne(y/scale), the quotient off by at most 1.5 units in fp32's
