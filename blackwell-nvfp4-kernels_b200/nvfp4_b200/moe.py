@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .dual_gemm import check_sf_perm, on_device
+from .dual_gemm import _current_stream_handle, check_sf_perm, on_device
 from .gemv import DTYPES, _empty, _launch, _rows_last
 
 
@@ -171,6 +171,7 @@ class ExpertWeights:
         self.sfb_ptrs = arr(*[s.data_ptr() for _, s in self.w])
         self.device = b0.device
         self._table = None
+        self._streams: set = set()  # whose calls the allocator knows to read the table
         self.space: dict = {}       # workspace bytes by (tokens, topk, type and alignment of x)
 
     def table(self) -> torch.Tensor:
@@ -184,7 +185,17 @@ class ExpertWeights:
             with torch.cuda.device(self.device):
                 _lib.check(lib.nvfp4_moe_table(self.b_ptrs, self.sfb_ptrs, len(self.w), self.n, self.k, host))
                 self._table = torch.frombuffer(host, dtype=torch.uint8).to(self.device)
+                self._streams.add(_current_stream_handle(self.device.index))
         return self._table
+
+    def _address(self, stream: int) -> int:
+        """The table's address for a call on the current stream (its handle).  The allocator is told of each stream but
+        the one that made the table, so that a table dropped before such a call has run stays until it has."""
+        table = self.table()
+        if stream not in self._streams:
+            table.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(stream)
+        return table.data_ptr()
 
     def __len__(self):
         return len(self.w)
@@ -278,9 +289,10 @@ def _products(x, expert_ids, w, w2, out, out_dtype):
         size = w.space[(tokens, topk, code, aligned)] = lib.nvfp4_moe_gemv_workspace_bytes(
             code, aligned and (tokens <= 2 or rows <= len(w)), tokens, topk, k)
     space = _empty((size,), (1,), dtype=torch.uint8, device=x.device) if size else None
+    stream = _current_stream_handle(x.device.index)
     _launch(lib.nvfp4_moe_gemv, x.device, (
-        px, code, ldx, x.shape[0] == rows and topk > 1, ids.data_ptr(), tokens, topk, w.table().data_ptr(),
-        w2.table().data_ptr() if w2 is not None else None, len(w), out.data_ptr(), DTYPES[out.dtype],
+        px, code, ldx, x.shape[0] == rows and topk > 1, ids.data_ptr(), tokens, topk, w._address(stream),
+        w2._address(stream) if w2 is not None else None, len(w), out.data_ptr(), DTYPES[out.dtype],
         ldo if ldo > n else n, n, k, space.data_ptr() if size else None, size))
     return out
 

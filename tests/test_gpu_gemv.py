@@ -603,6 +603,28 @@ def test_moe_gemv_repeated_experts_with_and_without_space(tokens, topk, e, n, k,
     assert _lib.device_status() == 0
 
 
+def test_expert_table_is_kept_for_calls_on_other_streams():
+    """Dropped while a call on another stream is still to read it, the table's memory is not handed out again."""
+    packed, atoms, dense = raw_weights(256, 128, seed=1, l=2)
+    pairs = list(zip(packed, atoms))
+    x, ids = torch.randn(2, 128, device="cuda").half(), torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    for form in (moe.gemv, lambda x, ids, w: moe.dual_gemv(x, ids, w, w)):
+        w = moe.ExpertWeights(pairs)
+        at, size = w.table().data_ptr(), w.table().numel()
+        want = form(x, ids, w)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)                # about 0.1 s
+            got = form(x, ids, w)
+        del w
+        fresh = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(64)]     # never written
+        busy = not side.query()
+        assert busy and at not in {t.data_ptr() for t in fresh}
+        side.synchronize()
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("tokens", [2, 12])
 def test_moe_gemv_table_rewritten_in_place(tokens):
     """Another table at the same address: its descriptors count, not the ones that a call before has read.
